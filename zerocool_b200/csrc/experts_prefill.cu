@@ -41,6 +41,7 @@
 // Every wait is bounded: after ~2^22 polls a role sets ZC_STATUS_TIMEOUT, raises the CTA's abort flag and
 // leaves its loop; the CTA then frees its TMEM and exits.
 #include "common.cuh"
+#include "tcgen05.cuh"
 #include <type_traits>
 
 namespace zc {
@@ -52,74 +53,8 @@ constexpr int PF_M = 128;
 constexpr int PF_NMAX = 64;           // tokens per tile (the N of the MMA, padded to 16)
 constexpr uint32_t PF_A_BYTES = PF_M * 128;          // one matrix, one stage: 128 rows x 64 halves
 constexpr uint32_t PF_B_BYTES = PF_NMAX * 128;
-constexpr uint32_t PF_POLL_LIMIT = 1u << 20;     // attempts of a bounded wait (each suspends for at most ~1 us: about one second in all)
 
 struct PfTile { int32_t expert, row0, rows, shared; };
-
-__device__ __forceinline__ uint32_t pf_smem(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(pf_smem(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pf_smem(bar)) : "memory");
-}
-// One attempt: mbarrier.try_wait suspends the thread until the phase completes or the time hint (1 us) passes
-// (it wakes as soon as the barrier flips, unlike a poll followed by a sleep).
-__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(pf_smem(bar)), "r"(parity), "r"(1000u) : "memory");       // suspend for at most ~1 us per attempt
-    return ok != 0;
-}
-// Bounded wait. Returns false (and raises the abort flag) when the phase did not complete in time or
-// another role has already given up.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {       // non-blocking probe
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(pf_smem(bar)), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t limit = PF_POLL_LIMIT) {
-    if (mbar_test(bar, parity)) return true;          // the common case in a pipeline that runs ahead
-    for (uint32_t i = 0; i < limit; ++i) {
-        if (mbar_try(bar, parity)) return true;
-        if (*abort_flag) return false;
-    }
-    *abort_flag = 1;
-    atomicOr(status, ZC_STATUS_TIMEOUT);
-    return false;
-}
-
-// The same for the lane that feeds the tensor cores: it has nothing else to do, and the wake-up of a suspended wait
-// (a few hundred clocks) is idle tensor time, so it polls without suspending. Still bounded.
-__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t limit = PF_POLL_LIMIT) {
-    for (uint32_t i = 0; i < (limit << 4); ++i) {
-        if (mbar_test(bar, parity)) return true;
-        if ((i & 1023u) == 1023u && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    atomicOr(status, ZC_STATUS_TIMEOUT);
-    return false;
-}
-
-// K-major, no swizzle: start address, LBO = 128 B (next k chunk), SBO = sbo bytes (next 8 rows), version 1.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr, uint32_t sbo = 1024) {
-    return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(128 >> 4) << 16) | (uint64_t(sbo >> 4) << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(pf_smem(bar)) : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr) : "memory");
-}
 
 // Position inside a block of eight k values at which value k%8 = i is stored: blocks hold
 // (k0,k4,k1,k5,k2,k6,k3,k7), the order the Q4 extraction below produces.
@@ -319,8 +254,8 @@ __global__ void __launch_bounds__(PF_THREADS, NMAT == 1 ? 2 : 1) prefill_kernel(
     const uint32_t N = uint32_t(tile.rows), Npad = (N + 15) & ~15u;
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t r0 = blockIdx.x * PF_M;
-    const uint32_t base = (pf_smem(pf_raw_smem) + 1023) & ~1023u;
-    uint8_t* const sm = pf_raw_smem + (base - pf_smem(pf_raw_smem));       // the same place as a generic pointer
+    const uint32_t base = (smem_addr(pf_raw_smem) + 1023) & ~1023u;
+    uint8_t* const sm = pf_raw_smem + (base - smem_addr(pf_raw_smem));       // the same place as a generic pointer
     auto at = [&](uint32_t shared_addr) { return sm + (shared_addr - base); };
     const uint32_t b_ring = base + S::A_RING, raw_base = b_ring + S::b_ring(D), meta_base = raw_base + S::raw_bytes(D);
     const uint32_t meta_sbo = (2 * G / 8) * 128, meta_tile = 128 * 2 * G * 2;      // A' tile of one matrix
@@ -348,7 +283,7 @@ __global__ void __launch_bounds__(PF_THREADS, NMAT == 1 ? 2 : 1) prefill_kernel(
     uint32_t ncols = 32;
     while (ncols < PF_ACC * NMAT * Npad) ncols <<= 1;     // PF_ACC accumulator buffers of NMAT x Npad columns
     if (warp == 4) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pf_smem(&tmem_base_s)), "r"(ncols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(ncols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -704,8 +639,8 @@ __global__ void __launch_bounds__(PW_THREADS, 1) prefill_wide_kernel(Call c, con
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t r0 = blockIdx.x * (NMAT == 2 ? 128u : 256u);
     const PwSmem L(Gp, DR, BITS);
-    const uint32_t base = (pf_smem(pf_raw_smem) + 1023) & ~1023u;
-    uint8_t* const sm = pf_raw_smem + (base - pf_smem(pf_raw_smem));
+    const uint32_t base = (smem_addr(pf_raw_smem) + 1023) & ~1023u;
+    uint8_t* const sm = pf_raw_smem + (base - smem_addr(pf_raw_smem));
     auto at = [&](uint32_t shared_addr) { return sm + (shared_addr - base); };
     const uint32_t b_ring = base + L.b_ring, raw_base = base + L.raw, meta_base = base + L.meta;
     const uint32_t meta_sbo = (2 * Gp / 8) * 128, meta_tile = 128 * 2 * Gp * 2;
@@ -730,7 +665,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) prefill_wide_kernel(Call c, con
         }
     }
     if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pf_smem(&tmem_base_s)), "r"(PW_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(PW_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -994,7 +929,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) prefill_wide_kernel(Call c, con
         if (abort_flag) {
             if (lane == 0) umma_commit(&drain_bar);
             __syncwarp();
-            if (warp == 8) for (uint32_t i = 0; i < PF_POLL_LIMIT && !mbar_try(&drain_bar, 0); ++i) {}
+            if (warp == 8) for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain_bar, 0); ++i) {}
             __syncwarp();
         }
         if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(PW_TMEM_COLS) : "memory");
@@ -1069,7 +1004,7 @@ __global__ void __launch_bounds__(96) pf_wait_selftest_kernel(uint32_t polls, ui
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (threadIdx.x == 0) { mbar_init(&never, 1); abort_flag = 0; asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pf_smem(&tmem_slot)), "r"(32u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(32u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

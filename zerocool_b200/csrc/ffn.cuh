@@ -1,0 +1,68 @@
+// What the dense feed-forward operators (include/zc_ffn.h) share: the microscaled format and the checks of their arguments.
+#pragma once
+#include "common.cuh"
+#include "../../include/zc_ffn.h"
+
+namespace zc {
+
+// ---------------------------------------------------------------------------------------------
+// Microscaled values
+// ---------------------------------------------------------------------------------------------
+inline uint64_t mx4_scale_bytes(uint32_t rows, uint32_t cols) { return uint64_t((uint64_t(rows) + 127) / 128) * ((uint64_t(cols) + 127) / 128) * 512; }
+// Byte of the scale of (row, block of 32 columns); ktiles = ceil(cols / 128).
+__host__ __device__ inline uint64_t mx4_scale_at(uint32_t row, uint32_t block, uint32_t ktiles) {
+    return (uint64_t(row / 128) * ktiles + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4;
+}
+#ifdef __CUDACC__
+// Scale byte of a block whose largest magnitude has these bits: floor(log2) - 2 from the exponent field (zero and subnormal values:
+// the smallest scale), 255 where a value is infinite or NaN.
+__device__ __forceinline__ uint32_t mx4_scale(uint32_t top_bits) {
+    const uint32_t field = top_bits >> 23;
+    return field == 255 ? 255u : field > 2 ? field - 2 : 0u;
+}
+__device__ __forceinline__ float mx4_factor(uint32_t s) { return __uint_as_float(s == 255 ? 0x7fc00000u : s ? s << 23 : 0x00400000u); }   // 2^(s - 127)
+// Eight values -> eight codes, the first in the lowest bits. 2^(127 - s) is exact for every s that mx4_scale gives (0..252).
+__device__ __forceinline__ uint32_t mx4_codes8(const float (&v)[8], uint32_t s) {
+    const float f = __uint_as_float((254u - s) << 23);
+    uint32_t word;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(word) : "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f), "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f));
+    return s == 255 ? 0u : word;
+}
+__device__ __forceinline__ float2 mx4_values2(uint32_t byte) {      // low half first
+    uint32_t h2;
+    asm("{\n\t.reg .b8 a, z;\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tmov.b16 {a, z}, h;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h2) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h2));
+}
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+#endif
+
+// ---------------------------------------------------------------------------------------------
+// Arguments
+// ---------------------------------------------------------------------------------------------
+struct Span { const void* p; uint64_t bytes; };
+inline bool overlap(const Span& a, const Span& b) {
+    const char *x = static_cast<const char*>(a.p), *y = static_cast<const char*>(b.p);
+    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+inline uint64_t dtype_bytes(int dtype) { return dtype == ZC_F32 ? 4 : 2; }
+inline uint64_t matrix_bytes(int dtype, uint64_t rows, uint64_t cols, uint64_t ld) { return rows ? ((rows - 1) * ld + cols) * dtype_bytes(dtype) : 0; }
+inline bool misaligned(const void* p, uintptr_t to = 16) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+// Whether every row of a matrix starts on 16 bytes.
+inline bool rows16(const void* p, uint64_t ld, uint64_t elem) { return !misaligned(p) && ld * elem % 16 == 0; }
+
+constexpr uint32_t MAX_COLS = 1u << 20;      // columns of any matrix here; rows are limited to 2^31 - 1 (TMA coordinates are signed)
+// A microscaled matrix: pointers (needed where rows > 0), alignment, sizes.
+int check_mx4(const char* who, const void* codes, const void* scales, uint32_t rows, uint32_t cols);
+// A plain matrix: type, row stride, and alignment to 16 bytes (rows and all: `tma`) or to its elements.
+int check_matrix(const char* who, const void* p, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, bool tma);
+
+int launch_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s);
+
+}  // namespace zc

@@ -1,0 +1,179 @@
+// Microscaled 4-bit matrices: quantisation, the way back, and row-major scales into tiles (include/zc_ffn.h has the format).
+//
+// All three are bound by memory: a value is read once (2 or 4 bytes) and 17/32 byte written, or the other way round. Nothing is
+// rounded but the value itself: the scale is a power of two, so x 2^-e is exact in FP32 wherever it does not fall below half of the
+// smallest e2m1 value's threshold, and the conversion instruction rounds it to nearest, ties to even.
+#include "ffn.cuh"
+
+namespace zc {
+namespace {
+
+constexpr int QT_ROWS = 128, QT_COLS = 256;     // one CTA: a row of two scale tiles
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+
+// Eight consecutive values of a row. VEC: the row is 16-byte aligned.
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (VEC) {
+        T raw[8];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) * 8 / 16; ++i) reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
+    }
+}
+
+// A CTA takes 128 rows x 256 columns, so that it writes whole scale tiles (gathered in shared memory; bytes past the last row or
+// column are written 0). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of the 256, a warp walks its 16 rows
+// four at a time (four independent 16-byte loads in flight per lane for 16-bit values, eight for FP32).
+template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t cols, uint64_t ld,
+                                                                                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    __shared__ __align__(16) uint8_t tile[2][512];
+    const uint32_t row0 = blockIdx.x * QT_ROWS, col0 = blockIdx.y * QT_COLS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t col = col0 + lane * 8;
+    if (threadIdx.x < 64) reinterpret_cast<uint4*>(tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
+    for (uint32_t r0 = warp * 4; r0 < n; r0 += 32) {
+        float v[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool live = r0 + i < n && col < cols;      // cols is a multiple of 32: the four lanes of a block agree
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            if (live) load8<T, VEC>(x + uint64_t(row0 + r0 + i) * ld + col, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t top = 0;                                // magnitudes as integers: ordered like the values, NaN above all
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t s = mx4_scale(top);
+            const uint32_t word = mx4_codes8(v[i], s);
+            if (r0 + i < n && col < cols) {
+                const uint32_t r = r0 + i;
+                *reinterpret_cast<uint32_t*>(codes + uint64_t(row0 + r) * (cols >> 1) + (col >> 1)) = word;
+                if ((lane & 3) == 0) tile[lane >> 4][(r & 31) * 16 + (r >> 5) * 4 + ((lane >> 2) & 3)] = uint8_t(s);
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t tiles = (cols + 127) / 128, t = blockIdx.y * 2 + (threadIdx.x >> 5);
+    if (threadIdx.x < 64 && t < tiles)
+        reinterpret_cast<uint4*>(scales + (uint64_t(blockIdx.x) * tiles + t) * 512)[threadIdx.x & 31] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+}
+
+// Eight values per thread.
+template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows,
+                                                                                        uint32_t cols, T* __restrict__ out, uint64_t ld) {
+    const uint32_t per_row = cols / 8;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(rows) * per_row; i += uint64_t(gridDim.x) * 256) {
+        const uint32_t row = uint32_t(i / per_row), col = uint32_t(i % per_row) * 8, block = col / 32;
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
+        const float f = mx4_factor(__ldg(scales + mx4_scale_at(row, block, (cols + 127) / 128)));
+        T v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 p = mx4_values2((word >> (8 * j)) & 0xffu);
+            v[2 * j] = from_f32<T>(p.x * f);
+            v[2 * j + 1] = from_f32<T>(p.y * f);
+        }
+        T* to = out + uint64_t(row) * ld + col;
+        if constexpr (VEC) {
+#pragma unroll
+            for (uint32_t j = 0; j < sizeof(T) * 8 / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[j] = v[j];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restrict__ from, uint32_t rows, uint32_t blocks, uint8_t* __restrict__ to) {
+    const uint32_t row = blockIdx.x * 128 + threadIdx.x, b0 = blockIdx.y * 4;
+    uint32_t word = 0;
+    for (uint32_t j = 0; j < 4; ++j)
+        if (row < rows && b0 + j < blocks) word |= uint32_t(from[uint64_t(row) * blocks + b0 + j]) << (8 * j);
+    *reinterpret_cast<uint32_t*>(to + (uint64_t(blockIdx.x) * gridDim.y + blockIdx.y) * 512 + (threadIdx.x & 31) * 16 + (threadIdx.x >> 5) * 4) = word;
+}
+
+template <typename T> void quantize_as(const void* x, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
+    const dim3 grid((rows + QT_ROWS - 1) / QT_ROWS, (cols + QT_COLS - 1) / QT_COLS);
+    auto* p = static_cast<const T*>(x);
+    auto *c = static_cast<uint8_t*>(codes), *sc = static_cast<uint8_t*>(scales);
+    if (rows16(x, ld, sizeof(T))) quantize_kernel<T, true><<<grid, 256, 0, s>>>(p, rows, cols, ld, c, sc);
+    else quantize_kernel<T, false><<<grid, 256, 0, s>>>(p, rows, cols, ld, c, sc);
+}
+template <typename T> void dequantize_as(const void* codes, const void* scales, uint32_t rows, uint32_t cols, void* out, uint64_t ld, cudaStream_t s) {
+    const uint64_t blocks = (uint64_t(rows) * (cols / 8) + 255) / 256;
+    const uint32_t grid = uint32_t(blocks < 148 * 32 ? blocks : 148 * 32);
+    auto *c = static_cast<const uint8_t*>(codes), *sc = static_cast<const uint8_t*>(scales);
+    if (rows16(out, ld, sizeof(T))) dequantize_kernel<T, true><<<grid, 256, 0, s>>>(c, sc, rows, cols, static_cast<T*>(out), ld);
+    else dequantize_kernel<T, false><<<grid, 256, 0, s>>>(c, sc, rows, cols, static_cast<T*>(out), ld);
+}
+
+}  // namespace
+
+int launch_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
+    if (dtype == ZC_BF16) quantize_as<__nv_bfloat16>(x, rows, cols, ld, codes, scales, s);
+    else if (dtype == ZC_F16) quantize_as<__half>(x, rows, cols, ld, codes, scales, s);
+    else quantize_as<float>(x, rows, cols, ld, codes, scales, s);
+    return check_launch(nullptr, "mx4 quantisation");
+}
+}  // namespace zc
+
+using namespace zc;
+
+extern "C" {
+
+int zc_mx4_scale_bytes(uint32_t rows, uint32_t cols, uint64_t* bytes) {
+    if (!bytes) return fail(nullptr, ZC_EINVAL, "missing buffer");
+    *bytes = mx4_scale_bytes(rows, cols);
+    return ZC_OK;
+}
+
+int zc_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, void* stream) {
+    int rc = check_mx4("zc_mx4_quantize", codes, scales, rows, cols);
+    if (rc == ZC_OK) rc = check_matrix("zc_mx4_quantize: x", x, dtype, rows, cols, ld, false);
+    if (rc != ZC_OK) return rc;
+    if (!rows) return ZC_OK;
+    const Span xs{x, matrix_bytes(dtype, rows, cols, ld)}, cs{codes, uint64_t(rows) * cols / 2}, ss{scales, mx4_scale_bytes(rows, cols)};
+    if (overlap(cs, xs) || overlap(ss, xs) || overlap(cs, ss)) return fail(nullptr, ZC_EINVAL, "zc_mx4_quantize: overlapping buffers");
+    return launch_mx4_quantize(x, dtype, rows, cols, ld, codes, scales, static_cast<cudaStream_t>(stream));
+}
+
+int zc_mx4_dequantize(const void* codes, const void* scales, uint32_t rows, uint32_t cols, void* out, int dtype, uint64_t ld, void* stream) {
+    int rc = check_mx4("zc_mx4_dequantize", codes, scales, rows, cols);
+    if (rc == ZC_OK) rc = check_matrix("zc_mx4_dequantize: out", out, dtype, rows, cols, ld, false);
+    if (rc != ZC_OK) return rc;
+    if (!rows) return ZC_OK;
+    const Span os{out, matrix_bytes(dtype, rows, cols, ld)}, cs{codes, uint64_t(rows) * cols / 2}, ss{scales, mx4_scale_bytes(rows, cols)};
+    if (overlap(cs, os) || overlap(ss, os)) return fail(nullptr, ZC_EINVAL, "zc_mx4_dequantize: overlapping buffers");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == ZC_BF16) dequantize_as<__nv_bfloat16>(codes, scales, rows, cols, out, ld, s);
+    else if (dtype == ZC_F16) dequantize_as<__half>(codes, scales, rows, cols, out, ld, s);
+    else dequantize_as<float>(codes, scales, rows, cols, out, ld, s);
+    return check_launch(nullptr, "mx4 dequantisation");
+}
+
+int zc_mx4_tile_scales(const void* row_scales, uint32_t rows, uint32_t cols, void* scales, void* stream) {
+    const int rc = check_mx4("zc_mx4_tile_scales", scales, scales, rows, cols);
+    if (rc != ZC_OK) return rc;
+    if (!rows) return ZC_OK;
+    if (!row_scales) return fail(nullptr, ZC_EINVAL, "zc_mx4_tile_scales: missing buffer");
+    if (overlap({row_scales, uint64_t(rows) * (cols / 32)}, {scales, mx4_scale_bytes(rows, cols)}))
+        return fail(nullptr, ZC_EINVAL, "zc_mx4_tile_scales: overlapping buffers");
+    tile_scales_kernel<<<dim3((rows + 127) / 128, (cols + 127) / 128), 128, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(row_scales), rows, cols / 32, static_cast<uint8_t*>(scales));
+    return check_launch(nullptr, "mx4 scale tiling");
+}
+
+}  // extern "C"

@@ -1,0 +1,267 @@
+"""Dense feed-forward operators on top of the C ABI (include/zc_ffn.h): microscaled 4-bit matrices and the gated block in 16 bits with
+its gradient - the shared or dense form of the block whose routed form is ``zerocool_b200.moe``.
+
+    w = mx4_quantize(weight)                  # once: codes and scales, 17/32 byte a value
+    h = mx4_gated(x, gate, up)                # silu(x gate^T) * (x up^T), one kernel
+    y = mx4_linear(h, down)                   # x of a product: plain (quantised on the way) or an Mx4
+
+    h, g, u = gated_forward(x, gate, up, save=True)
+    dx, dgate, dup = gated_backward(dh, x, gate, up, g, u)
+
+Calls run on the tensors' device and torch's current stream of it, allocate results and scratch with torch and may be captured into a
+CUDA graph (after one call outside a capture). Nothing here has a CPU path. Errors are those of ``zerocool_b200.moe``: ``ValueError``
+for arguments, ``RuntimeError`` for the device.
+"""
+import ctypes
+
+from . import moe
+from .records import BF16, F16, F32
+
+EXPORTS = ["zc_mx4_scale_bytes", "zc_mx4_quantize", "zc_mx4_dequantize", "zc_mx4_tile_scales", "zc_mx4_linear", "zc_mx4_gated",
+           "zc_gated_forward", "zc_gated_backward", "zc_ffn_status"]
+
+_lib = None
+
+
+def load_library():
+    """The library of ``zerocool_b200.moe`` with the prototypes of include/zc_ffn.h."""
+    global _lib
+    if _lib is None:
+        lib = moe.load_library()
+        vp, u32, u64, i32 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int
+        lib.zc_mx4_scale_bytes.argtypes = [u32, u32, ctypes.POINTER(u64)]
+        lib.zc_mx4_quantize.argtypes = [vp, i32, u32, u32, u64, vp, vp, vp]
+        lib.zc_mx4_dequantize.argtypes = [vp, vp, u32, u32, vp, i32, u64, vp]
+        lib.zc_mx4_tile_scales.argtypes = [vp, u32, u32, vp, vp]
+        lib.zc_mx4_linear.argtypes = [vp, i32, u64, vp, vp, u32, u32, vp, vp, u32, vp, i32, u64, vp]
+        lib.zc_mx4_gated.argtypes = [vp, i32, u64, vp, vp, u32, u32, vp, vp, vp, vp, u32, vp, i32, u64, vp]
+        lib.zc_gated_forward.argtypes = [vp, u64, vp, vp, i32, u32, u32, u32, vp, vp, vp, vp]
+        lib.zc_gated_backward.argtypes = [vp, u64, vp, u64, vp, vp, vp, vp, i32, u32, u32, u32, vp, vp, vp, vp, vp, vp]
+        lib.zc_ffn_status.argtypes = [vp, ctypes.POINTER(u32)]
+        _lib = lib
+    return _lib
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _code(dtype, sixteen=False):
+    torch = _torch()
+    codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+    if dtype not in codes or (sixteen and dtype == torch.float32):
+        raise ValueError(f"dtype must be {'bfloat16 or float16' if sixteen else 'bfloat16, float16 or float32'}, not {dtype}")
+    return codes[dtype]
+
+
+def _matrix(name, t, shape=None, dtype=None, contiguous=False):
+    """Checks a matrix operand; -> its row stride in elements."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name} must have consecutive columns and rows that do not overlap")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _same_device(device, **others):
+    for name, t in others.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _call(device, name, *args):
+    """One library call on the device's current stream (its last argument)."""
+    torch = _torch()
+    lib = load_library()
+    with torch.cuda.device(device):
+        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != moe.ZC_OK:
+        moe._raise(rc, lib.zc_last_error())
+
+
+def _scale_bytes(rows, cols):
+    return -(-rows // 128) * -(-cols // 128) * 512
+
+
+def _out(out, rows, cols, dtype, device, name="out"):
+    """The output matrix and its row stride."""
+    if out is None:
+        out = _torch().empty((rows, cols), dtype=dtype, device=device)
+        return out, cols
+    ld = _matrix(name, out, (rows, cols), dtype)
+    _same_device(device, **{name: out})
+    return out, ld
+
+
+class Mx4:
+    """A microscaled matrix [rows, cols]: codes uint8 [rows, cols / 2] and scales uint8 [ceil(rows / 128) ceil(cols / 128) 512] in the
+    tile layout of include/zc_ffn.h. Holds the tensors; copies nothing."""
+
+    def __init__(self, codes, scales):
+        torch = _torch()
+        if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
+            raise ValueError("codes must be contiguous uint8 [rows, cols / 2], cols a multiple of 32")
+        if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.device != codes.device or \
+                scales.numel() != _scale_bytes(codes.shape[0], codes.shape[1] * 2):
+            raise ValueError("scales must be contiguous uint8 of the codes' device, 512 for each 128 rows x 128 columns")
+        if not codes.is_cuda:
+            raise ValueError("codes must be on a CUDA device")
+        self.codes, self.scales = codes, scales
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def cols(self):
+        return self.codes.shape[1] * 2
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @staticmethod
+    def empty(rows, cols, device):
+        torch = _torch()
+        return Mx4(torch.empty((rows, cols // 2), dtype=torch.uint8, device=device), torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))
+
+
+def mx4_quantize(x, out=None):
+    """x [rows, cols] (bfloat16, float16 or float32, cols a multiple of 32) -> Mx4; ``out``: an Mx4 of that shape to write."""
+    ld = _matrix("x", x)
+    rows, cols = x.shape
+    if not cols or cols % 32:
+        raise ValueError("columns must be a multiple of 32")
+    if out is None:
+        out = Mx4.empty(rows, cols, x.device)
+    elif (out.rows, out.cols) != (rows, cols):
+        raise ValueError(f"out must be [{rows}, {cols}]")
+    _same_device(x.device, out=out)
+    _call(x.device, "zc_mx4_quantize", x.data_ptr(), _code(x.dtype), rows, cols, ld, out.codes.data_ptr(), out.scales.data_ptr())
+    return out
+
+
+def mx4_dequantize(q, dtype=None, out=None):
+    """The values of an Mx4 (default bfloat16, which holds each of them exactly)."""
+    torch = _torch()
+    dtype = out.dtype if dtype is None and out is not None else dtype or torch.bfloat16
+    code = _code(dtype)
+    out, ld = _out(out, q.rows, q.cols, dtype, q.device)
+    _call(q.device, "zc_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, out.data_ptr(), code, ld)
+    return out
+
+
+def mx4_from_rows(codes, scales):
+    """A checkpoint's codes [rows, cols / 2] and row-major scales [rows, cols / 32] (both uint8) -> Mx4 (the codes are not copied)."""
+    torch = _torch()
+    if scales.dim() != 2 or scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], codes.shape[-1] // 16):
+        raise ValueError("scales must be contiguous uint8 [rows, cols / 32]")
+    q = Mx4(codes, torch.empty(_scale_bytes(codes.shape[0], codes.shape[1] * 2), dtype=torch.uint8, device=codes.device))
+    _same_device(codes.device, scales=scales)
+    _call(codes.device, "zc_mx4_tile_scales", scales.data_ptr(), q.rows, q.cols, q.scales.data_ptr())
+    return q
+
+
+def _mx4_product(entry, x, weights, out_dtype, out):
+    torch = _torch()
+    w = weights[0]
+    device, cols, rows = w.device, w.cols, w.rows
+    for other in weights[1:]:
+        if (other.rows, other.cols) != (rows, cols):
+            raise ValueError(f"the weights differ in shape: [{rows}, {cols}] and [{other.rows}, {other.cols}]")
+        _same_device(device, weights=other)
+    if isinstance(x, Mx4):
+        tokens, xcols, plain = x.rows, x.cols, (None, F32, 0)
+        q = x
+    else:
+        ld = _matrix("x", x)
+        (tokens, xcols), plain = x.shape, (x.data_ptr(), _code(x.dtype), ld)
+        q = None
+    if xcols != cols:
+        raise ValueError(f"x has {xcols} columns, the weights {cols}")
+    _same_device(device, x=x)
+    out_dtype = out.dtype if out_dtype is None and out is not None else out_dtype or torch.bfloat16
+    code = _code(out_dtype)
+    out, out_ld = _out(out, tokens, rows, out_dtype, device)
+    if q is None:
+        q = Mx4.empty(tokens, cols, device)
+    pointers = [p for m in weights for p in (m.codes.data_ptr(), m.scales.data_ptr())]
+    _call(device, entry, *plain, q.codes.data_ptr(), q.scales.data_ptr(), tokens, cols, *pointers, rows, out.data_ptr(), code, out_ld)
+    return out
+
+
+def mx4_linear(x, w, out_dtype=None, out=None):
+    """x w^T [tokens, w.rows] in out_dtype (default bfloat16): x an Mx4 or a plain matrix [tokens, w.cols], w an Mx4."""
+    return _mx4_product("zc_mx4_linear", x, [w], out_dtype, out)
+
+
+def mx4_gated(x, gate, up, out_dtype=None, out=None):
+    """silu(x gate^T) * (x up^T) [tokens, ffn] in out_dtype (default bfloat16): x as in mx4_linear, gate and up Mx4 [ffn, cols]."""
+    return _mx4_product("zc_mx4_gated", x, [gate, up], out_dtype, out)
+
+
+def gated_forward(x, gate, up, save=False, out=None):
+    """silu(x gate^T) * (x up^T): x [tokens, hidden], gate and up [ffn, hidden], one of bfloat16 and float16; -> h [tokens, ffn], and
+    with ``save`` (h, g, u): the two products as gated_backward wants them."""
+    torch = _torch()
+    code = _code(getattr(x, "dtype", None), sixteen=True)
+    ld = _matrix("x", x)
+    (tokens, hidden), ffn = x.shape, gate.shape[0]
+    for name, w in (("gate", gate), ("up", up)):
+        _matrix(name, w, (ffn, hidden), x.dtype, contiguous=True)
+    _same_device(x.device, gate=gate, up=up)
+    if out is None:
+        out = torch.empty((tokens, ffn), dtype=x.dtype, device=x.device)
+    else:
+        _matrix("out", out, (tokens, ffn), x.dtype, contiguous=True)
+        _same_device(x.device, out=out)
+    g, u = (torch.empty_like(out), torch.empty_like(out)) if save else (None, None)
+    _call(x.device, "zc_gated_forward", x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), code, tokens, hidden, ffn, out.data_ptr(),
+          g.data_ptr() if save else None, u.data_ptr() if save else None)
+    return (out, g, u) if save else out
+
+
+def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
+    """The gradient of gated_forward -> (dx, dgate, dup) in the operands' dtype (None for what is not asked for)."""
+    torch = _torch()
+    code = _code(getattr(x, "dtype", None), sixteen=True)
+    x_ld = _matrix("x", x)
+    (tokens, hidden), ffn = x.shape, gate.shape[0]
+    for name, w in (("gate", gate), ("up", up)):
+        _matrix(name, w, (ffn, hidden), x.dtype, contiguous=True)
+    dh_ld = _matrix("dh", dh, (tokens, ffn), x.dtype)
+    for name, t in (("g", g), ("u", u)):
+        _matrix(name, t, (tokens, ffn), x.dtype, contiguous=True)
+    _same_device(x.device, dh=dh, gate=gate, up=up, g=g, u=u)
+    if not input_grad and not weight_grads:
+        return None, None, None
+    dg, du = torch.empty_like(g), torch.empty_like(u)
+    dx = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device) if input_grad else None
+    dgate, dup = (torch.empty_like(gate), torch.empty_like(up)) if weight_grads else (None, None)
+    pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _call(x.device, "zc_gated_backward", dh.data_ptr(), dh_ld, x.data_ptr(), x_ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), code,
+          tokens, hidden, ffn, dg.data_ptr(), du.data_ptr(), pointer(dx), pointer(dgate), pointer(dup))
+    return dx, dgate, dup
+
+
+def status(device=None):
+    """Waits for the device's current stream and returns (then clears) the device's status word of these operators."""
+    torch = _torch()
+    word = ctypes.c_uint32()
+    lib = load_library()
+    with torch.cuda.device(device):
+        rc = lib.zc_ffn_status(torch.cuda.current_stream().cuda_stream, ctypes.byref(word))
+    if rc != moe.ZC_OK:
+        moe._raise(rc, lib.zc_last_error())
+    return word.value
