@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_s;
+    pdl_wait();
+    pdl_launch_dependents();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -260,10 +262,268 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few tokens
+// ---------------------------------------------------------------------------------------------
+// D[M, tokens] = W . X^T: the weights are the 128 rows of a product, the tokens (at most 256, padded to a multiple of 16) its columns, so
+// a single token costs the tensor cores an eighth of what 128 would and the launch is what its bytes are: the weights, once. A CTA owns
+// one tile of 128 weight rows (of gate and of up) and one run of blocks of K; the CTAs of a cluster share a tile's K and add their partial
+// sums through distributed shared memory, in the order of their ranks. The lanes of the epilogue hold consecutive output columns of
+// a token, so plain stores are coalesced whatever the row stride.
+// x given plain: every CTA quantises its own part of the tokens' K into shared memory (the epilogue warps, while the weights arrive),
+// in the swizzle TMA would have written. The kernel before may still run while this one starts (programmatic launch): until it has
+// ended nothing is read but into L2, where a later write of it would arrive too.
+constexpr uint32_t FEW_THREADS = 192, FEW_STAGES = 8;
+constexpr uint32_t FEW_TOKENS = 128;
+constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_SMEM_MAX = 226 * 1024;      // what a ring may take (two CTAs an SM); the most a CTA may have
+constexpr uint32_t FEW_PLAIN_TOKENS = 32, FEW_PLAIN_BYTES = 32 * 1024;    // x is quantised inside up to these
+constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
+
+struct FewPlan {
+    uint32_t M, tokens, n;              // weight rows, tokens, tokens padded
+    uint32_t splits, kown;              // CTAs of a cluster, blocks of K of each
+    uint32_t kblocks, segs, ksteps;     // blocks of a segment, segments, steps of a segment's last block
+    uint32_t stages, stage, resident;   // ring; byte offset of the quantised tokens (0: they come through the ring)
+    uint32_t smem;
+    uint32_t tmem_columns, sf_column, sf_columns;
+    uint32_t prefetch;                  // blocks of K to request into L2 ahead
+    uint32_t idesc, ktiles;
+    const uint8_t *sfw[2], *sfx;
+    const void* x;
+    uint64_t x_ld;
+    uint32_t x_dtype, cols;
+    bool x_vec;
+    void *out, *g, *u;
+    uint64_t ldo;
+    int out_type;
+};
+
+__device__ __forceinline__ void store_one(void* out, int type, uint64_t at, float v) {
+    if (type == ZC_BF16) static_cast<__nv_bfloat16*>(out)[at] = from_f32<__nv_bfloat16>(v);
+    else if (type == ZC_F16) static_cast<__half*>(out)[at] = from_f32<__half>(v);
+    else static_cast<float*>(out)[at] = v;
+}
+template <bool GATED> __device__ __forceinline__ void few_store(const FewPlan& p, uint64_t at, float a, float b) {
+    if constexpr (GATED) {
+        if (p.g) { store_one(p.g, p.out_type, at, a); store_one(p.u, p.out_type, at, b); }
+        a = silu(a) * b;
+    }
+    store_one(p.out, p.out_type, at, a);
+}
+__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void load8_any(const FewPlan& p, uint64_t at, float (&v)[8]) {
+    if (p.x_dtype == ZC_BF16) p.x_vec ? load8<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(p.x) + at, v) : load8<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(p.x) + at, v);
+    else if (p.x_dtype == ZC_F16) p.x_vec ? load8<__half, true>(static_cast<const __half*>(p.x) + at, v) : load8<__half, false>(static_cast<const __half*>(p.x) + at, v);
+    else p.x_vec ? load8<float, true>(static_cast<const float*>(p.x) + at, v) : load8<float, false>(static_cast<const float*>(p.x) + at, v);
+}
+
+template <bool MX4, bool A_MN, int MATS>
+__global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant__ TileMaps maps, const FewPlan p) {
+    constexpr uint32_t KB = MX4 ? 128 : 64;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[FEW_STAGES], empty[FEW_STAGES], acc_full, tokens_ready, drain;
+    __shared__ uint32_t tmem_s, abort_s;
+    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* const ring_p = raw + (ring - smem_addr(raw));
+    const uint32_t rank = blockIdx.x % p.splits, m0 = blockIdx.x / p.splits * TILE_M;
+    const uint32_t k0 = rank * p.kown, k1 = min(k0 + p.kown, p.kblocks * p.segs);
+    const bool fused = p.resident != 0;
+    uint32_t* const status = &ffn_status_word;
+    volatile uint32_t* const abort_flag = &abort_s;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&acc_full, 1);
+        mbar_init(&tokens_ready, 128);
+        mbar_init(&drain, 1);
+        abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_s)), "r"(p.tmem_columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 0 && lane == 0) {
+        for (uint32_t k = k0; k < min(k0 + p.prefetch, k1); ++k) {
+            const uint32_t seg = k / p.kblocks, kb = k % p.kblocks;
+            for (uint32_t i = 0; i < MATS; ++i) {
+                if constexpr (A_MN) {
+                    prefetch_2d(&maps.a[seg], m0, kb * 64);
+                    if (m0 + 64 < p.M) prefetch_2d(&maps.a[seg], m0 + 64, kb * 64);
+                } else {
+                    prefetch_2d(&maps.a[i], kb * KB, m0);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_s;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const uint32_t b_bytes = fused ? 0 : p.n * 128, xtiles = p.n > 128 ? 2 : 1;      // token rows of a stage; scale tiles of the tokens
+    const uint32_t sf_off = MATS * A_BYTES + b_bytes;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t k = k0; k < k1; ++k, ++it) {
+                const uint32_t slot = it % p.stages, a = ring + slot * p.stage, seg = k / p.kblocks, kb = k % p.kblocks;
+                if (it >= p.stages && !mbar_wait(&empty[slot], (it / p.stages - 1) & 1, abort_flag, status)) { ok = false; break; }
+                const uint32_t atoms = MX4 ? min(2u, p.ktiles - kb * 2) : 0;
+                const bool two = xtiles == 2 && p.tokens > 128;
+                mbar_expect(&full[slot], MATS * A_BYTES + b_bytes + atoms * 512 * (MATS + (fused ? 0 : two ? 2 : 1)));
+                for (uint32_t i = 0; i < MATS; ++i) {
+                    if constexpr (A_MN) {
+                        tma_load_2d(a, &maps.a[seg], &full[slot], m0, kb * 64);
+                        tma_load_2d(a + 8192, &maps.a[seg], &full[slot], m0 + 64, kb * 64);
+                    } else {
+                        tma_load_2d(a + i * A_BYTES, &maps.a[i], &full[slot], kb * KB, m0);
+                    }
+                    if constexpr (MX4) bulk_load(a + sf_off + i * 1024, p.sfw[i] + (uint64_t(m0 / 128) * p.ktiles + kb * 2) * 512, atoms * 512, &full[slot]);
+                }
+                if (!fused) {
+                    tma_load_2d(a + MATS * A_BYTES, &maps.b[seg], &full[slot], kb * KB, 0);
+                    if constexpr (MX4) {
+                        bulk_load(a + sf_off + MATS * 1024, p.sfx + uint64_t(kb) * 1024, atoms * 512, &full[slot]);
+                        if (two) bulk_load(a + sf_off + MATS * 1024 + 1024, p.sfx + (uint64_t(p.ktiles) + kb * 2) * 512, atoms * 512, &full[slot]);
+                    }
+                }
+            }
+            if (!ok)
+                for (uint32_t f = it > p.stages ? it - p.stages : 0; f < it; ++f)
+                    for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&full[f % p.stages], (f / p.stages) & 1); ++i) {}
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status);
+            uint32_t it = 0, more = 0;
+            for (uint32_t k = k0; ok && k < k1; ++k, ++it) {
+                const uint32_t slot = it % p.stages, a = ring + slot * p.stage, kb = k % p.kblocks;
+                if (!mbar_wait(&full[slot], (it / p.stages) & 1, abort_flag, status)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t b = fused ? ring + p.resident + it * (p.n * 128 + 1024) : a + MATS * A_BYTES;
+                const uint32_t sfb = fused ? b + p.n * 128 : a + sf_off + MATS * 1024;
+                const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4, sf = tmem + p.sf_column + slot * p.sf_columns;
+                const uint64_t db = desc_at(DESC_K_MAJOR, b);
+                if constexpr (MX4) {
+                    for (uint32_t j = 0; j < (steps + 1) / 2; ++j) {
+                        for (uint32_t i = 0; i < MATS; ++i) tmem_copy_scales(sf + i * 8 + j * 4, desc_at(DESC_SCALES, a + sf_off + i * 1024 + j * 512));
+                        for (uint32_t i = 0; i < xtiles; ++i) tmem_copy_scales(sf + MATS * 8 + j * 4 * xtiles + i * 4, desc_at(DESC_SCALES, sfb + i * 1024 + j * 512));
+                    }
+                }
+                for (uint32_t s = 0; s < steps; ++s, more = 1) {
+                    for (uint32_t i = 0; i < MATS; ++i) {
+                        const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a + i * A_BYTES);
+                        if constexpr (MX4) {
+                            const uint32_t id = (s & 1) * 2;
+                            umma_mx4(tmem + i * p.n, da + s * 2, db + s * 2, p.idesc | id << 29 | id << 4, sf + i * 8 + (s >> 1) * 4, sf + MATS * 8 + (s >> 1) * 4 * xtiles, more);
+                        } else {
+                            umma_f16(tmem + i * p.n, da + s * (A_MN ? 128 : 2), db + s * 2, p.idesc, more);
+                        }
+                    }
+                }
+                umma_commit(&empty[slot]);
+            }
+            if (ok) umma_commit(&acc_full);
+            else {
+                umma_commit(&drain);
+                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        if (MX4 && fused) {
+            // Four lanes share a block of 32 values; the padding rows stay as they are (their columns are not stored), the columns past the
+            // last one become zero codes with a zero scale byte.
+            const uint32_t groups = (k1 - k0) * 32, tid = threadIdx.x - 64;            // groups of eight columns of this CTA's K
+            for (uint32_t i = tid; i < p.tokens * groups; i += 128) {
+                const uint32_t t = i / groups, c = i % groups, col = k0 * 256 + c * 8;
+                float v[8] = {};
+                if (col < p.cols) load8_any(p, uint64_t(t) * p.x_ld + col, v);
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const uint32_t s = mx4_scale(top), block = c / 32, in = c % 32;       // in: which eight of the block's 256 columns
+                uint8_t* const b = ring_p + p.resident + block * (p.n * 128 + 1024);
+                *reinterpret_cast<uint32_t*>(b + t * 128 + (((in >> 2) ^ (t & 7)) << 4) + (in & 3) * 4) = mx4_codes8(v, s);
+                if ((in & 3) == 0) b[p.n * 128 + (in >> 4) * 512 + (t & 31) * 16 + (t >> 5) * 4 + ((in >> 2) & 3)] = uint8_t(s);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&tokens_ready);
+        }
+        const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, abort_flag, status));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float* const part = reinterpret_cast<float*>(ring_p);        // [matrix][token][row]: every stage has been read when the products are done
+        for (uint32_t t0 = 0; ok && t0 < p.tokens; t0 += 16) {
+            uint32_t v[MATS][16];
+#pragma unroll
+            for (uint32_t i = 0; i < MATS; ++i) tmem_ld16(tmem + (quarter << 21) + i * p.n + t0, v[i]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) {
+                if (t0 + j >= p.tokens) break;
+                if (p.splits > 1) {
+#pragma unroll
+                    for (uint32_t i = 0; i < MATS; ++i) part[(i * p.tokens + t0 + j) * 128 + row] = __uint_as_float(v[i][j]);
+                } else if (m0 + row < p.M) {
+                    few_store<MATS == 2>(p, uint64_t(t0 + j) * p.ldo + m0 + row, __uint_as_float(v[0][j]), __uint_as_float(v[MATS - 1][j]));
+                }
+            }
+            __syncwarp();
+        }
+    }
+    if (p.splits > 1) {
+        cluster_sync();
+        if (warp >= 2 && !*abort_flag) {
+            const uint32_t row = threadIdx.x - 64;
+            for (uint32_t t = rank; t < p.tokens; t += p.splits) {
+                if (m0 + row >= p.M) break;
+                float v[MATS];
+#pragma unroll
+                for (uint32_t i = 0; i < MATS; ++i) {
+                    float each[8];
+#pragma unroll
+                    for (uint32_t r = 0; r < 8; ++r)
+                        if (r < p.splits) each[r] = load_peer(ring + ((i * p.tokens + t) * 128 + row) * 4, r);
+                    v[i] = each[0];
+#pragma unroll
+                    for (uint32_t r = 1; r < 8; ++r)
+                        if (r < p.splits) v[i] += each[r];
+                }
+                few_store<MATS == 2>(p, uint64_t(t) * p.ldo + m0 + row, v[0], v[MATS - 1]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();          // no CTA leaves while another may still read its sums
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
+}
+
 // dg = dh u s (1 + g (1 - s)), du = dh g s; eight values a thread. Bound by memory: three reads and two writes of 16 bits a value.
 template <typename T> __global__ void __launch_bounds__(256) gated_gradient_kernel(const T* __restrict__ dh, uint64_t dh_ld, const T* __restrict__ g, const T* __restrict__ u, uint32_t tokens,
                                                                                    uint32_t ffn, T* __restrict__ dg, T* __restrict__ du) {
     const uint32_t per_row = ffn / 8;
+    pdl_wait();
+    pdl_launch_dependents();
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(tokens) * per_row; i += uint64_t(gridDim.x) * 256) {
         const uint64_t row = i / per_row, col = i % per_row;
         alignas(16) T a[8], b[8], c[8], d[8], e[8];
@@ -305,16 +565,18 @@ bool make_map(CUtensorMap& m, const void* base, bool bytes, uint64_t inner, uint
     return encode(&m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, elem,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-bool map_codes(CUtensorMap& m, const void* codes, uint32_t rows, uint32_t cols) { return make_map(m, codes, true, cols / 2, rows, cols / 2, 128); }
-// A 16-bit operand [rows, cols]: K along its rows (boxes of 64 k x 128 rows), or across them (boxes of 64 columns x 64 k).
-bool map_rows(CUtensorMap& m, const void* p, uint32_t rows, uint32_t cols, uint64_t ld, bool k_across) { return make_map(m, p, false, cols, rows, ld * 2, k_across ? 64 : 128); }
+bool map_codes(CUtensorMap& m, const void* codes, uint32_t rows, uint32_t cols, uint32_t box) { return make_map(m, codes, true, cols / 2, rows, cols / 2, box); }
+// A 16-bit operand [rows, cols]: K along its rows (boxes of 64 k x 128 rows, or of so many), or across them (boxes of 64 columns x 64 k).
+bool map_rows(CUtensorMap& m, const void* p, uint32_t rows, uint32_t cols, uint64_t ld, bool k_across, uint32_t box = TILE_M) {
+    return make_map(m, p, false, cols, rows, ld * 2, k_across ? 64 : box);
+}
 
 // Instruction descriptors. Both: N / 8 from bit 17, M / 16 from bit 24.
-uint32_t idesc_f16(int dtype, bool a_mn, bool b_mn) {      // FP32 accumulators; operand types; which operand has M / N along its rows
+uint32_t idesc_f16(int dtype, bool a_mn, bool b_mn, uint32_t n = TILE_N) {      // FP32 accumulators; operand types; which operand has M / N along its rows
     const uint32_t t = dtype == ZC_BF16 ? 1 : 0;
-    return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | ((TILE_N / 8) << 17) | ((TILE_M / 16) << 24);
+    return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | ((n / 8) << 17) | ((TILE_M / 16) << 24);
 }
-uint32_t idesc_mx4() { return (1u << 7) | (1u << 10) | ((TILE_N / 8) << 17) | (1u << 23) | ((TILE_M / 16) << 24); }      // e2m1 both, e8m0 scales
+uint32_t idesc_mx4(uint32_t n = TILE_N) { return (1u << 7) | (1u << 10) | ((n / 8) << 17) | (1u << 23) | ((TILE_M / 16) << 24); }      // e2m1 both, e8m0 scales
 
 struct Device { int index = -1; uint32_t sms = 0; };
 int current_device(Device& d) {
@@ -330,13 +592,25 @@ int current_device(Device& d) {
     return ZC_OK;
 }
 
+// The opt-in to large shared memory of one kernel, once per device.
+struct Configured {
+    std::atomic<bool> done[MAX_DEVICES] = {};
+    template <typename Kernel> int once(Kernel kernel, int device, size_t smem) {
+        if (done[device].load(std::memory_order_relaxed)) return ZC_OK;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e)); }
+        done[device].store(true, std::memory_order_relaxed);
+        return ZC_OK;
+    }
+};
+
 template <bool MX4, bool A_MN, bool B_MN, bool GATED> int launch_tiles(const TileMaps& maps, TilePlan& p, cudaStream_t s) {
     Device d;
-    const int rc = current_device(d);
+    int rc = current_device(d);
     if (rc != ZC_OK) return rc;
+    static Configured configured;
     auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(TileSmem<MX4>::bytes));
-    if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e)); }
+    if ((rc = configured.once(kernel, d.index, TileSmem<MX4>::bytes)) != ZC_OK) return rc;
     constexpr uint32_t width = GATED ? TILE_N / 2 : TILE_N;
     p.mtiles = (p.M + TILE_M - 1) / TILE_M;
     p.ntiles = (p.N + width - 1) / width;
@@ -344,14 +618,50 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED> int launch_tiles(const Til
     if (tiles > 0x7fffffffu) return fail(nullptr, ZC_EINVAL, "too many output tiles");
     p.tiles = uint32_t(tiles);
     p.vec = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && (!p.out[1] || rows16(p.out[1], p.ldo, dtype_bytes(p.out_type)));
-    kernel<<<p.tiles < d.sms ? p.tiles : d.sms, THREADS, TileSmem<MX4>::bytes, s>>>(maps, p);
-    return check_launch(nullptr, "dense product");
+    return launched(launch_after(kernel, dim3(p.tiles < d.sms ? p.tiles : d.sms), THREADS, TileSmem<MX4>::bytes, 1, s, maps, p), "dense product");
 }
 
-void set_k(TilePlan& p, uint32_t k, uint32_t block) {
+template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block) {
     p.kblocks = (k + block - 1) / block;
     const uint32_t left = k - (p.kblocks - 1) * block, step = block / 4;
     p.ksteps = (left + step - 1) / step;
+}
+
+// Cuts a call of few tokens (at most FEW_TOKENS). kblocks, ksteps, segs, M, tokens, cols are set; plain: x is to be quantised.
+void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
+    p.n = (p.tokens + 15) / 16 * 16;
+    const uint32_t total = p.kblocks * p.segs, mtiles = (p.M + TILE_M - 1) / TILE_M;
+    uint32_t splits = sms / mtiles;
+    splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
+    if (splits > total) splits = total;
+    p.kown = (total + splits - 1) / splits;
+    p.splits = (total + p.kown - 1) / p.kown;
+    const uint32_t quantised = p.kown * (p.n * 128 + 1024), xtiles = p.n > 128 ? 2 : 1;
+    const bool fused = plain && p.tokens <= FEW_PLAIN_TOKENS && quantised <= FEW_PLAIN_BYTES;
+    p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? xtiles * 1024 : 0));
+    const uint32_t room = FEW_SMEM - 1024 - (fused ? quantised : 0);
+    p.stages = room / p.stage;
+    if (p.stages > FEW_STAGES) p.stages = FEW_STAGES;
+    if (p.stages > p.kown) p.stages = p.kown;
+    uint32_t bytes = p.stages * p.stage;
+    const uint32_t sums = p.splits > 1 ? mats * p.tokens * 512 : 0;
+    if (!fused && bytes < sums) bytes = sums;
+    p.resident = fused ? (bytes > sums ? bytes : (sums + 1023) / 1024 * 1024) : 0;
+    p.smem = 1024 + (fused ? p.resident + quantised : bytes);
+    p.sf_column = mats * p.n;
+    p.sf_columns = mx4 ? mats * 8 + 8 * xtiles : 0;
+    p.tmem_columns = 32;
+    while (p.tmem_columns < p.sf_column + p.stages * p.sf_columns) p.tmem_columns *= 2;
+    const uint64_t ahead = FEW_AHEAD / (uint64_t(mtiles) * p.splits * mats * A_BYTES);
+    p.prefetch = ahead < p.kown ? uint32_t(ahead) : p.kown;
+}
+
+template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, FewPlan& p, const Device& d, cudaStream_t s) {
+    static Configured configured;
+    auto kernel = few_kernel<MX4, A_MN, MATS>;
+    const int rc = configured.once(kernel, d.index, FEW_SMEM_MAX);
+    if (rc != ZC_OK) return rc;
+    return launched(launch_after(kernel, dim3((p.M + TILE_M - 1) / TILE_M * p.splits), FEW_THREADS, p.smem, p.splits, s, maps, p), "dense product of few tokens");
 }
 
 int no_maps() { return fail(nullptr, ZC_EEXEC, "the driver did not encode a tensor map"); }
@@ -375,12 +685,33 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
             bad = bad || overlap(os, t) || (x && (overlap(cs, t) || overlap(ss, t)));
     if (bad) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x && (rc = launch_mx4_quantize(x, x_dtype, tokens, cols, x_ld, x_codes, x_scales, s)) != ZC_OK) return rc;
+    Device d;
+    if ((rc = current_device(d)) != ZC_OK) return rc;
     TileMaps maps{};
+    if (tokens <= FEW_TOKENS) {
+        FewPlan p{};
+        p.M = rows; p.tokens = tokens; p.segs = 1;
+        set_k(p, cols, 256);
+        plan_few(p, true, mats, x != nullptr, d.sms);
+        if (x && !p.resident && (rc = launch_mx4_quantize(x, x_dtype, tokens, cols, x_ld, x_codes, x_scales, s)) != ZC_OK) return rc;
+        for (int i = 0; i < mats; ++i) {
+            if (!map_codes(maps.a[i], w[i].codes, rows, cols, TILE_M)) return no_maps();
+            p.sfw[i] = static_cast<const uint8_t*>(w[i].scales);
+        }
+        if (!p.resident && !map_codes(maps.b[0], x_codes, tokens, cols, p.n)) return no_maps();
+        p.idesc = idesc_mx4(p.n);
+        p.ktiles = (cols + 127) / 128;
+        p.sfx = static_cast<const uint8_t*>(x_scales);
+        p.x = x; p.x_ld = x_ld; p.x_dtype = x_dtype; p.cols = cols;
+        p.x_vec = x && rows16(x, x_ld, dtype_bytes(x_dtype));
+        p.out = out; p.ldo = out_ld; p.out_type = out_dtype;
+        return mats == 2 ? launch_few<true, false, 2>(maps, p, d, s) : launch_few<true, false, 1>(maps, p, d, s);
+    }
+    if (x && (rc = launch_mx4_quantize(x, x_dtype, tokens, cols, x_ld, x_codes, x_scales, s)) != ZC_OK) return rc;
     TilePlan p{};
-    if (!map_codes(maps.a[0], x_codes, tokens, cols)) return no_maps();
+    if (!map_codes(maps.a[0], x_codes, tokens, cols, TILE_M)) return no_maps();
     for (int i = 0; i < mats; ++i)
-        if (!map_codes(maps.b[i], w[i].codes, rows, cols)) return no_maps();
+        if (!map_codes(maps.b[i], w[i].codes, rows, cols, TILE_M)) return no_maps();
     p.M = tokens; p.N = rows; p.segs = 1; p.outs = 1;
     set_k(p, cols, 256);
     p.idesc = idesc_mx4();
@@ -434,6 +765,19 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
         for (int j = 0; j < i; ++j) if (overlap(to[i], to[j])) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
     }
     TileMaps maps{};
+    if (tokens <= FEW_TOKENS) {
+        Device d;
+        if ((rc = current_device(d)) != ZC_OK) return rc;
+        FewPlan p{};
+        p.M = ffn; p.tokens = tokens; p.segs = 1;
+        set_k(p, hidden, 64);
+        plan_few(p, false, 2, false, d.sms);
+        if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, false) || !map_rows(maps.a[1], up, ffn, hidden, hidden, false) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, false, p.n))
+            return no_maps();
+        p.idesc = idesc_f16(dtype, false, false, p.n);
+        p.out = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
+        return launch_few<false, false, 2>(maps, p, d, static_cast<cudaStream_t>(stream));
+    }
     TilePlan p{};
     if (!map_rows(maps.a[0], x, tokens, hidden, x_ld, false) || !map_rows(maps.b[0], gate, ffn, hidden, hidden, false) || !map_rows(maps.b[1], up, ffn, hidden, hidden, false))
         return no_maps();
@@ -473,15 +817,26 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     }
     const uint64_t blocks = (uint64_t(tokens) * (ffn / 8) + 255) / 256;
     const uint32_t grid = uint32_t(blocks < 148 * 16 ? blocks : 148 * 16);
-    if (dtype == ZC_BF16) {
-        typedef __nv_bfloat16 T;
-        gated_gradient_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(dh), dh_ld, static_cast<const T*>(g), static_cast<const T*>(u), tokens, ffn, static_cast<T*>(dg), static_cast<T*>(du));
-    } else {
-        typedef __half T;
-        gated_gradient_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(dh), dh_ld, static_cast<const T*>(g), static_cast<const T*>(u), tokens, ffn, static_cast<T*>(dg), static_cast<T*>(du));
-    }
-    if ((rc = check_launch(nullptr, "gated gradient")) != ZC_OK) return rc;
-    if (dx) {
+    const auto gradient = [&](auto kernel, auto type) {
+        typedef decltype(type) T;
+        return launch_after(kernel, dim3(grid), 256, 0, 1, s, static_cast<const T*>(dh), dh_ld, static_cast<const T*>(g), static_cast<const T*>(u), tokens, ffn, static_cast<T*>(dg), static_cast<T*>(du));
+    };
+    rc = launched(dtype == ZC_BF16 ? gradient(gated_gradient_kernel<__nv_bfloat16>, __nv_bfloat16()) : gradient(gated_gradient_kernel<__half>, __half()), "gated gradient");
+    if (rc != ZC_OK) return rc;
+    if (dx && tokens <= FEW_TOKENS) {
+        Device d;
+        if ((rc = current_device(d)) != ZC_OK) return rc;
+        TileMaps maps{};
+        FewPlan p{};
+        p.M = hidden; p.tokens = tokens; p.segs = 2;
+        set_k(p, ffn, 64);
+        plan_few(p, false, 1, false, d.sms);
+        if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, true) || !map_rows(maps.a[1], up, ffn, hidden, hidden, true) ||
+            !map_rows(maps.b[0], dg, tokens, ffn, ffn, false, p.n) || !map_rows(maps.b[1], du, tokens, ffn, ffn, false, p.n)) return no_maps();
+        p.idesc = idesc_f16(dtype, true, false, p.n);
+        p.out = dx; p.ldo = hidden; p.out_type = dtype;
+        if ((rc = launch_few<false, true, 1>(maps, p, d, s)) != ZC_OK) return rc;
+    } else if (dx) {
         TileMaps maps{};
         TilePlan p{};
         if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, false) || !map_rows(maps.a[1], du, tokens, ffn, ffn, false) ||

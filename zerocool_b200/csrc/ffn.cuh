@@ -41,6 +41,24 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+
+// Eight consecutive values of a row. VEC: the row is 16-byte aligned.
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (VEC) {
+        T raw[8];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) * 8 / 16; ++i) reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
+    }
+}
 #endif
 
 // ---------------------------------------------------------------------------------------------
@@ -62,6 +80,28 @@ constexpr uint32_t MAX_COLS = 1u << 20;      // columns of any matrix here; rows
 int check_mx4(const char* who, const void* codes, const void* scales, uint32_t rows, uint32_t cols);
 // A plain matrix: type, row stride, and alignment to 16 bytes (rows and all: `tma`) or to its elements.
 int check_matrix(const char* who, const void* p, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, bool tma);
+
+#ifdef __CUDACC__
+// A launch that may start while the kernel before it on the stream still runs (the rules of launch_chained: everything up to pdl_wait()
+// reads and writes no global memory, and pdl_launch_dependents() comes after it). `cluster`: CTAs of a cluster.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, uint32_t block, size_t smem, uint32_t cluster, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+inline int launched(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return ZC_OK;
+    cudaGetLastError();
+    return fail(nullptr, ZC_EEXEC, std::string("CUDA launch of ") + what + ": " + cudaGetErrorString(e));
+}
+#endif
 
 int launch_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s);
 

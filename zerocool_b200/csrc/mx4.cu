@@ -10,25 +10,6 @@ namespace {
 
 constexpr int QT_ROWS = 128, QT_COLS = 256;     // one CTA: a row of two scale tiles
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32(float v) { return v; }
-
-// Eight consecutive values of a row. VEC: the row is 16-byte aligned.
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    if constexpr (VEC) {
-        T raw[8];
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) * 8 / 16; ++i) reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
-    }
-}
-
 // A CTA takes 128 rows x 256 columns, so that it writes whole scale tiles (gathered in shared memory; bytes past the last row or
 // column are written 0). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of the 256, a warp walks its 16 rows
 // four at a time (four independent 16-byte loads in flight per lane for 16-bit values, eight for FP32).
@@ -39,6 +20,8 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_
     const uint32_t col = col0 + lane * 8;
     if (threadIdx.x < 64) reinterpret_cast<uint4*>(tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
     const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
     for (uint32_t r0 = warp * 4; r0 < n; r0 += 32) {
         float v[4][8];
@@ -75,6 +58,8 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_
 template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows,
                                                                                         uint32_t cols, T* __restrict__ out, uint64_t ld) {
     const uint32_t per_row = cols / 8;
+    pdl_wait();
+    pdl_launch_dependents();
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(rows) * per_row; i += uint64_t(gridDim.x) * 256) {
         const uint32_t row = uint32_t(i / per_row), col = uint32_t(i % per_row) * 8, block = col / 32;
         const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
@@ -100,33 +85,31 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantiz
 __global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restrict__ from, uint32_t rows, uint32_t blocks, uint8_t* __restrict__ to) {
     const uint32_t row = blockIdx.x * 128 + threadIdx.x, b0 = blockIdx.y * 4;
     uint32_t word = 0;
+    pdl_wait();
+    pdl_launch_dependents();
     for (uint32_t j = 0; j < 4; ++j)
         if (row < rows && b0 + j < blocks) word |= uint32_t(from[uint64_t(row) * blocks + b0 + j]) << (8 * j);
     *reinterpret_cast<uint32_t*>(to + (uint64_t(blockIdx.x) * gridDim.y + blockIdx.y) * 512 + (threadIdx.x & 31) * 16 + (threadIdx.x >> 5) * 4) = word;
 }
 
-template <typename T> void quantize_as(const void* x, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
+template <typename T> int quantize_as(const void* x, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
     const dim3 grid((rows + QT_ROWS - 1) / QT_ROWS, (cols + QT_COLS - 1) / QT_COLS);
-    auto* p = static_cast<const T*>(x);
-    auto *c = static_cast<uint8_t*>(codes), *sc = static_cast<uint8_t*>(scales);
-    if (rows16(x, ld, sizeof(T))) quantize_kernel<T, true><<<grid, 256, 0, s>>>(p, rows, cols, ld, c, sc);
-    else quantize_kernel<T, false><<<grid, 256, 0, s>>>(p, rows, cols, ld, c, sc);
+    auto kernel = rows16(x, ld, sizeof(T)) ? quantize_kernel<T, true> : quantize_kernel<T, false>;
+    return launched(launch_after(kernel, grid, 256, 0, 1, s, static_cast<const T*>(x), rows, cols, ld, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)), "mx4 quantisation");
 }
-template <typename T> void dequantize_as(const void* codes, const void* scales, uint32_t rows, uint32_t cols, void* out, uint64_t ld, cudaStream_t s) {
+template <typename T> int dequantize_as(const void* codes, const void* scales, uint32_t rows, uint32_t cols, void* out, uint64_t ld, cudaStream_t s) {
     const uint64_t blocks = (uint64_t(rows) * (cols / 8) + 255) / 256;
     const uint32_t grid = uint32_t(blocks < 148 * 32 ? blocks : 148 * 32);
-    auto *c = static_cast<const uint8_t*>(codes), *sc = static_cast<const uint8_t*>(scales);
-    if (rows16(out, ld, sizeof(T))) dequantize_kernel<T, true><<<grid, 256, 0, s>>>(c, sc, rows, cols, static_cast<T*>(out), ld);
-    else dequantize_kernel<T, false><<<grid, 256, 0, s>>>(c, sc, rows, cols, static_cast<T*>(out), ld);
+    auto kernel = rows16(out, ld, sizeof(T)) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+    return launched(launch_after(kernel, dim3(grid), 256, 0, 1, s, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, static_cast<T*>(out), ld), "mx4 dequantisation");
 }
 
 }  // namespace
 
 int launch_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
-    if (dtype == ZC_BF16) quantize_as<__nv_bfloat16>(x, rows, cols, ld, codes, scales, s);
-    else if (dtype == ZC_F16) quantize_as<__half>(x, rows, cols, ld, codes, scales, s);
-    else quantize_as<float>(x, rows, cols, ld, codes, scales, s);
-    return check_launch(nullptr, "mx4 quantisation");
+    if (dtype == ZC_BF16) return quantize_as<__nv_bfloat16>(x, rows, cols, ld, codes, scales, s);
+    if (dtype == ZC_F16) return quantize_as<__half>(x, rows, cols, ld, codes, scales, s);
+    return quantize_as<float>(x, rows, cols, ld, codes, scales, s);
 }
 }  // namespace zc
 
@@ -158,10 +141,9 @@ int zc_mx4_dequantize(const void* codes, const void* scales, uint32_t rows, uint
     const Span os{out, matrix_bytes(dtype, rows, cols, ld)}, cs{codes, uint64_t(rows) * cols / 2}, ss{scales, mx4_scale_bytes(rows, cols)};
     if (overlap(cs, os) || overlap(ss, os)) return fail(nullptr, ZC_EINVAL, "zc_mx4_dequantize: overlapping buffers");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == ZC_BF16) dequantize_as<__nv_bfloat16>(codes, scales, rows, cols, out, ld, s);
-    else if (dtype == ZC_F16) dequantize_as<__half>(codes, scales, rows, cols, out, ld, s);
-    else dequantize_as<float>(codes, scales, rows, cols, out, ld, s);
-    return check_launch(nullptr, "mx4 dequantisation");
+    if (dtype == ZC_BF16) return dequantize_as<__nv_bfloat16>(codes, scales, rows, cols, out, ld, s);
+    if (dtype == ZC_F16) return dequantize_as<__half>(codes, scales, rows, cols, out, ld, s);
+    return dequantize_as<float>(codes, scales, rows, cols, out, ld, s);
 }
 
 int zc_mx4_tile_scales(const void* row_scales, uint32_t rows, uint32_t cols, void* scales, void* stream) {
@@ -171,9 +153,8 @@ int zc_mx4_tile_scales(const void* row_scales, uint32_t rows, uint32_t cols, voi
     if (!row_scales) return fail(nullptr, ZC_EINVAL, "zc_mx4_tile_scales: missing buffer");
     if (overlap({row_scales, uint64_t(rows) * (cols / 32)}, {scales, mx4_scale_bytes(rows, cols)}))
         return fail(nullptr, ZC_EINVAL, "zc_mx4_tile_scales: overlapping buffers");
-    tile_scales_kernel<<<dim3((rows + 127) / 128, (cols + 127) / 128), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const uint8_t*>(row_scales), rows, cols / 32, static_cast<uint8_t*>(scales));
-    return check_launch(nullptr, "mx4 scale tiling");
+    return launched(launch_after(tile_scales_kernel, dim3((rows + 127) / 128, (cols + 127) / 128), 128, 0, 1, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(row_scales), rows, cols / 32,
+                                 static_cast<uint8_t*>(scales)), "mx4 scale tiling");
 }
 
 }  // extern "C"
