@@ -8,11 +8,12 @@
 //     its dgate, dup                A = dg or du, B = x, both with K = tokens across the rows; the two outputs are tiles of one launch
 // Either type has 128 bytes of K per row and pipeline stage and four tensor-core steps of 32 bytes in it, so the loop is the same.
 //
-// A persistent CTA per SM walks 128 x 256 tiles: one thread issues TMA loads into a ring of four stages, one issues the products into
-// tensor memory, eight warps drain it, apply the epilogue in FP32 and store. 128 x 256 is the widest tile a single CTA can issue: a
-// step reads 12 KB of shared memory for 128 clocks of tensor work. 16-bit products alternate between two accumulators of 256 columns,
-// so the drain is hidden; MX4 products keep their scales in tensor memory too (32 columns a stage), which leaves one, and the drain
-// (all of it into registers before the first store) is what the next tile waits for.
+// A pair of CTAs (cta_group::2) walks tiles of 256 rows x 256 (or 128) columns: either CTA stages its 128 rows of A and its half of B's
+// rows by TMA into a ring, one thread of the leading CTA issues the products of both, and eight warps of either drain its 128 rows from
+// tensor memory, apply the epilogue in FP32 and store. The pair halves B's traffic: 32 KB from L2 per SM for 512 clocks of tensor work, not
+// the 48 KB of a single CTA's widest tile, whose loop L2 bounded (11 TB/s: 150 us for MX4 8192 x 8192 x 4096).
+// Two accumulators where they fit, so that the drain is hidden. MX4 products keep their scales in tensor memory too (32 columns a stage),
+// which leaves one of 256: the next tile waits until it is in registers, not until it is stored.
 // Every wait is bounded (POLL_LIMIT): one that runs out raises ZC_STATUS_TIMEOUT and the CTA's abort flag; its roles leave their
 // loops, wait for the copies and products in flight, and the tensor memory is freed.
 #include "ffn.cuh"
@@ -48,20 +49,20 @@ namespace {
 
 __device__ uint32_t ffn_status_word;     // the device's status word of these operators (zc_ffn_status)
 
-constexpr uint32_t TILE_M = 128, TILE_N = 256, STAGES = 4, THREADS = 320;
-constexpr uint32_t A_BYTES = TILE_M * 128, B_BYTES = TILE_N * 128, SF_BYTES = 3 * 1024;
-constexpr uint32_t SF_COLUMN = 256, SF_COLUMNS = 32;      // MX4: first column of the scales, columns a stage: A 2 x 4, B 2 x 8 (of 32)
+constexpr uint32_t TILE_M = 128, THREADS = 320;           // rows of a CTA
+constexpr uint32_t A_BYTES = TILE_M * 128;
+constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory columns of a stage's scales: A 2 x 4, B 2 x 8 at most
+constexpr uint32_t PATCH = 9;                              // floats of a row of the patch that a warp turns where rows are not aligned
 
-struct TileMaps { CUtensorMap a[2], b[2]; };
+struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2]; };
 
 struct TilePlan {
     uint32_t M, N;                      // rows and columns of an output (gated: N = ffn)
     uint32_t kblocks, ksteps;           // blocks of 128 bytes of K; steps of 32 bytes in the last one
     uint32_t segs, outs;                // pairs (a[s], b[s]) whose products add up; outputs a[z] . b[0]
-    uint32_t mtiles, ntiles, tiles;
+    uint32_t mtiles, ntiles, tiles;     // of 256 rows
     uint32_t idesc;
-    uint32_t ktiles, brows;             // MX4: scale tiles along K; rows of B
-    const uint8_t *sfa, *sfb[2];
+    uint32_t ktiles;                    // MX4: scale tiles along K
     void* out[2];
     uint64_t ldo;
     void *g, *u;                        // gated: where the two products go as well, or null
@@ -75,191 +76,226 @@ struct Tile { uint32_t z, m0, n0; };
 __device__ __forceinline__ Tile tile_at(const TilePlan& p, uint32_t t, uint32_t width) {
     const uint32_t per = p.mtiles * p.ntiles, z = t / per, i = t % per, band = i / (8 * p.ntiles), j = i % (8 * p.ntiles);
     const uint32_t rows = min(8u, p.mtiles - band * 8);
-    return {z, (band * 8 + j % rows) * TILE_M, j / rows * width};
+    return {z, (band * 8 + j % rows) * 2 * TILE_M, j / rows * width};
 }
 
-// `valid` leading values of v to a row.
-template <typename T, int NC> __device__ __forceinline__ void store_row(T* to, uint32_t valid, bool vec, const float (&v)[NC]) {
+// A warp's 32 rows (one a lane) of NC columns: `live`, the lane's row exists; `valid` leading columns do. Rows that are 16-byte aligned are
+// stored by their lanes, 16 bytes at a time. Others are turned eight columns at a time through a patch of shared memory, so that eight
+// lanes store consecutive columns (a lane's own row, value by value, would touch 32 sectors a store: 45 -> 25 us for 257 x 10007).
+template <typename T, int NC> __device__ __forceinline__ void store_rows(T* to, uint64_t ld, bool live, uint32_t valid, bool vec, float* patch, const float (&v)[NC]) {
     constexpr int PER = 16 / sizeof(T);
+    if (vec) {
+        if (!live) return;
 #pragma unroll
-    for (int c = 0; c < NC; c += PER) {
-        if (vec && c + PER <= valid) {
-            alignas(16) T w[PER];
+        for (int c = 0; c < NC; c += PER) {
+            if (c + PER <= valid) {
+                alignas(16) T w[PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j) w[j] = from_f32<T>(v[c + j]);
-            *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(w);
-        } else {
+                for (int j = 0; j < PER; ++j) w[j] = from_f32<T>(v[c + j]);
+                *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(w);
+            } else {
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (c + j < valid) to[c + j] = from_f32<T>(v[c + j]);
+                for (int j = 0; j < PER; ++j)
+                    if (c + j < valid) to[c + j] = from_f32<T>(v[c + j]);
+            }
         }
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 31, rows = __popc(__ballot_sync(0xffffffffu, live));
+    T* const first = to - lane * ld;
+#pragma unroll
+    for (int c = 0; c < NC; c += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) patch[lane * PATCH + j] = v[c + j];
+        __syncwarp();
+        const uint32_t col = c + (lane & 7);
+#pragma unroll
+        for (uint32_t r = lane >> 3; r < 32; r += 4)
+            if (r < rows && col < valid) first[r * ld + col] = from_f32<T>(patch[r * PATCH + (lane & 7)]);
+        __syncwarp();
     }
 }
-template <int NC> __device__ __forceinline__ void store_as(void* out, int type, uint64_t at, uint32_t valid, bool vec, const float (&v)[NC]) {
-    if (type == ZC_BF16) store_row(static_cast<__nv_bfloat16*>(out) + at, valid, vec, v);
-    else if (type == ZC_F16) store_row(static_cast<__half*>(out) + at, valid, vec, v);
-    else store_row(static_cast<float*>(out) + at, valid, vec, v);
+template <int NC> __device__ __forceinline__ void store_as(void* out, int type, uint64_t at, uint64_t ld, bool live, uint32_t valid, bool vec, float* patch, const float (&v)[NC]) {
+    if (type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out) + at, ld, live, valid, vec, patch, v);
+    else if (type == ZC_F16) store_rows(static_cast<__half*>(out) + at, ld, live, valid, vec, patch, v);
+    else store_rows(static_cast<float*>(out) + at, ld, live, valid, vec, patch, v);
 }
 __device__ __forceinline__ float silu(float v) { return __fdiv_rn(v, 1.0f + expf(-v)); }
 
-template <bool MX4> struct TileSmem {
-    static constexpr uint32_t stage = A_BYTES + B_BYTES + (MX4 ? SF_BYTES : 0), bytes = STAGES * stage + 1024;
+template <bool MX4, int N> struct TileSmem {
+    static constexpr uint32_t b = N / 2 * 128, stage = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), stages = 6, patches = 8 * 32 * PATCH * 4;
+    static constexpr uint32_t bytes = stages * stage + patches + 1024;
 };
 
-template <bool MX4, bool A_MN, bool B_MN, bool GATED>
+template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const TilePlan p) {
-    constexpr uint32_t ACC = MX4 ? 1 : 2, STAGE = TileSmem<MX4>::stage, KB = MX4 ? 128 : 64;      // KB: TMA elements of K a block (bytes of codes, 16-bit values)
-    constexpr uint32_t WIDTH = GATED ? TILE_N / 2 : TILE_N;
+    typedef TileSmem<MX4, N> Smem;
+    constexpr uint32_t STAGES = Smem::stages, STAGE = Smem::stage, ACC = MX4 && N == 256 ? 1 : 2, SF_COLUMN = ACC * N;
+    constexpr uint32_t KB = MX4 ? 128 : 64;               // TMA elements of K a block (bytes of codes, 16-bit values)
+    constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (uint32_t i = 0; i < ACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
+        for (uint32_t i = 0; i < ACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16); }
         mbar_init(&drain, 1);
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_s)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_s;
     pdl_wait();
     pdl_launch_dependents();
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
+        if (elect_one()) {
+            uint32_t it = 0, slot = 0, round = 0;
             bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+            for (uint32_t t = pair; ok && t < p.tiles; t += pairs) {
                 const Tile c = tile_at(p, t, WIDTH);
+                const int row = c.m0 + rank * TILE_M;                                       // of A
+                const int col = GATED ? c.n0 : c.n0 + rank * (N / 2);                       // row of B (gated: the leader has gate's, the other up's)
                 for (uint32_t s = 0; ok && s < p.segs; ++s) {
                     const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : s];
-                    const CUtensorMap* const mb = &maps.b[s];
+                    const CUtensorMap* const mb = &maps.b[GATED ? rank : s];
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++it) {
-                        const uint32_t slot = it % STAGES, a = ring + slot * STAGE, b = a + A_BYTES;
-                        if (it >= STAGES && !mbar_wait(&empty[slot], (it / STAGES - 1) & 1, abort_flag, status)) { ok = false; break; }
-                        const uint32_t atoms = MX4 ? min(2u, p.ktiles - kb * 2) : 0;
-                        const uint32_t second = GATED ? 0 : c.n0 + 128;      // MX4: row of B whose scale tile follows (gated: up's own)
-                        const bool two = GATED || second < p.brows;
-                        mbar_expect(&full[slot], A_BYTES + B_BYTES + atoms * 512 * (two ? 3 : 2));
+                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES;
+                        if (round && !mbar_wait_cluster(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
+                        const uint32_t bar = map_to(smem_addr(&full[slot]), 0);             // the leader counts the bytes of both
+                        if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
                         if constexpr (A_MN) {
-                            for (uint32_t i = 0; i < 2; ++i) tma_load_2d(a + i * 8192, ma, &full[slot], c.m0 + i * 64, kb * 64);
+                            for (uint32_t i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, ma, bar, row + i * 64, kb * 64);
                         } else {
-                            tma_load_2d(a, ma, &full[slot], kb * KB, c.m0);
+                            tma_load_2d_pair(a, ma, bar, kb * KB, row);
                         }
                         if constexpr (B_MN) {
-                            for (uint32_t i = 0; i < 4; ++i) tma_load_2d(b + i * 8192, mb, &full[slot], c.n0 + i * 64, kb * 64);
-                        } else if constexpr (GATED) {
-                            tma_load_2d(b, &maps.b[0], &full[slot], kb * KB, c.n0);
-                            tma_load_2d(b + 16384, &maps.b[1], &full[slot], kb * KB, c.n0);
+                            for (uint32_t i = 0; i < N / 128; ++i) tma_load_2d_pair(b + i * 8192, mb, bar, col + i * 64, kb * 64);
                         } else {
-                            tma_load_2d(b, mb, &full[slot], kb * KB, c.n0);
-                            tma_load_2d(b + 16384, mb, &full[slot], kb * KB, c.n0 + 128);
+                            tma_load_2d_pair(b, mb, bar, kb * KB, col);
                         }
-                        if constexpr (MX4) {
-                            const uint32_t sf = b + B_BYTES;
-                            const uint64_t at = uint64_t(c.n0 / 128) * p.ktiles + kb * 2;
-                            bulk_load(sf, p.sfa + (uint64_t(c.m0 / 128) * p.ktiles + kb * 2) * 512, atoms * 512, &full[slot]);
-                            bulk_load(sf + 1024, p.sfb[0] + at * 512, atoms * 512, &full[slot]);
-                            if (two) bulk_load(sf + 2048, GATED ? p.sfb[1] + at * 512 : p.sfb[0] + (at + p.ktiles) * 512, atoms * 512, &full[slot]);
+                        if constexpr (MX4) {      // two scale tiles (256 k) of this CTA's rows of A and of all rows of B
+                            const uint32_t sf = b + Smem::b;
+                            const int at = (c.n0 / 128) * p.ktiles + kb * 2;
+                            tma_load_2d_pair(sf, &maps.sfa, bar, 0, (row / 128) * p.ktiles + kb * 2);
+                            tma_load_2d_pair(sf + 1024, &maps.sfb[0], bar, 0, at);
+                            if (N == 256) tma_load_2d_pair(sf + 2048, &maps.sfb[GATED ? 1 : 0], bar, 0, GATED ? at : at + p.ktiles);
                         }
+                        if (++slot == STAGES) { slot = 0; ++round; }
                     }
                 }
             }
-            if (!ok)      // the last copies into every slot land before the CTA may end
-                for (uint32_t f = it > STAGES ? it - STAGES : 0; f < it; ++f)
-                    for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&full[f % STAGES], (f / STAGES) & 1); ++i) {}
+            if (!ok) {        // the last copies land before the CTA may end: the leader's barriers count those of both
+                if (rank == 0)
+                    for (uint32_t f = it > STAGES ? it - STAGES : 0; f < it; ++f)
+                        for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&full[f % STAGES], (f / STAGES) & 1); ++i) {}
+                else
+                    for (uint32_t i = 0; i < 2000; ++i) __nanosleep(1000);
+            }
         }
+        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t it = 0, n = 0;
+        if (rank == 0 && elect_one()) {
+            uint32_t n = 0, slot = 0, phase = 0;
             bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++n) {
-                const uint32_t buf = n % ACC, acc = tmem + buf * 256;
-                if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
+            for (uint32_t t = pair; ok && t < p.tiles; t += pairs, ++n) {
+                const uint32_t buf = n % ACC, acc = tmem + buf * N;
+                if (n >= ACC && !mbar_wait_cluster(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t more = 0;
                 for (uint32_t s = 0; ok && s < p.segs; ++s) {
-                    for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++it) {
-                        const uint32_t slot = it % STAGES, a = ring + slot * STAGE, b = a + A_BYTES;
-                        if (!mbar_wait(&full[slot], (it / STAGES) & 1, abort_flag, status)) { ok = false; break; }
+                    for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES;
+                        if (!mbar_wait_cluster(&full[slot], phase, abort_flag, status)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
                         const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4;
                         const uint32_t sf = tmem + SF_COLUMN + slot * SF_COLUMNS;
                         if constexpr (MX4) {
-                            // 128 k of scales: four columns for A's rows, eight for B's (its two blocks of 128 rows)
-                            for (uint32_t j = 0; j < (steps + 1) / 2; ++j) {
-                                tmem_copy_scales(sf + j * 4, desc_at(DESC_SCALES, b + B_BYTES + j * 512));
-                                tmem_copy_scales(sf + 8 + j * 8, desc_at(DESC_SCALES, b + B_BYTES + 1024 + j * 512));
-                                tmem_copy_scales(sf + 12 + j * 8, desc_at(DESC_SCALES, b + B_BYTES + 2048 + j * 512));
+                            // 128 k of scales: four columns for A's rows, four or eight for B's
+                            const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
+#pragma unroll
+                            for (uint32_t j = 0; j < 2; ++j) {
+                                if (j * 2 >= steps) break;
+                                tmem_copy_scales_pair(sf + j * 4, ds + j * 32);
+#pragma unroll
+                                for (uint32_t i = 0; i < N / 128; ++i) tmem_copy_scales_pair(sf + 8 + j * 8 + i * 4, ds + 64 * (i + 1) + j * 32);
                             }
                         }
-                        for (uint32_t k = 0; k < steps; ++k, more = 1) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            if (k >= steps) break;
                             if constexpr (MX4) {
-                                const uint32_t id = (k & 1) * 2;         // which two of a column's four scales
-                                umma_mx4(acc, da + k * 2, db + k * 2, p.idesc | id << 29 | id << 4, sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8, more);
+                                constexpr uint32_t odd = 2u << 29 | 2u << 4;      // the upper two of a column's four scales
+                                umma_mx4_pair(acc, da + k * 2, db + k * 2, k & 1 ? p.idesc | odd : p.idesc, sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8, more);
                             } else {
-                                umma_f16(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
+                                umma_f16_pair(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
                             }
+                            more = 1;
                         }
-                        umma_commit(&empty[slot]);
+                        umma_commit_pair(&empty[slot]);
+                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
                     }
                 }
-                if (ok) umma_commit(&acc_full[buf]);
+                if (ok) umma_commit_pair(&acc_full[buf]);
             }
             if (abort_s) {       // products in flight read shared memory and write tensor memory: they end first
-                umma_commit(&drain);
-                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
+                umma_commit_pair(&drain);
+                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try_cluster(&drain, 0); ++i) {}
             }
         }
+        __syncwarp();
     } else {
-        const uint32_t half = (warp - 2) >> 2, quarter = warp & 3;      // columns; the 32 lanes of tensor memory a warp can read
+        constexpr int COLS = WIDTH / 2;                                 // output columns of a warp
+        const uint32_t half = (warp - 2) >> 2, quarter = warp & 3;      // which columns; the 32 lanes of tensor memory a warp can read
+        float* const patch = reinterpret_cast<float*>(raw + (ring - smem_addr(raw)) + STAGES * STAGE) + (warp - 2) * 32 * PATCH;
         uint32_t n = 0;
-        for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
+        for (uint32_t t = pair; t < p.tiles; t += pairs, ++n) {
             const Tile c = tile_at(p, t, WIDTH);
-            const uint32_t buf = n % ACC, acc = tmem + buf * 256 + (quarter << 21);
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (n / ACC) & 1, abort_flag, status))) break;
+            const uint32_t buf = n % ACC, acc = tmem + buf * N + (quarter << 21);
+            if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[buf], (n / ACC) & 1, abort_flag, status))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float v[128];      // gated: 64 of gate, then 64 of up
+            float v[COLS], w[GATED ? COLS : 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(acc + (GATED ? (i >> 1) * 128 + half * 64 + (i & 1) * 32 : half * 128 + i * 32), v + i * 32);
+            for (int i = 0; i < COLS; i += 32) {
+                tmem_ld32(acc + half * COLS + i, v + i);
+                if constexpr (GATED) tmem_ld32(acc + N / 2 + half * COLS + i, w + i);
+            }
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            const uint32_t row = c.m0 + quarter * 32 + lane, col = c.n0 + half * (WIDTH / 2);
-            if (row >= p.M || col >= p.N) continue;
+            if (lane == 0) mbar_arrive_at(map_to(smem_addr(&acc_empty[buf]), 0));
+            const uint32_t row = c.m0 + rank * TILE_M + quarter * 32 + lane, col = c.n0 + half * COLS;
+            if (col >= p.N) continue;
             const uint64_t at = uint64_t(row) * p.ldo + col;
             const uint32_t valid = p.N - col;
+            const bool live = row < p.M;
             if constexpr (GATED) {
-                float gate[64], up[64];
-#pragma unroll
-                for (int i = 0; i < 64; ++i) { gate[i] = v[i]; up[i] = v[64 + i]; }
                 if (p.g) {
-                    store_as(p.g, p.out_type, at, valid, p.vec, gate);
-                    store_as(p.u, p.out_type, at, valid, p.vec, up);
+                    store_as(p.g, p.out_type, at, p.ldo, live, valid, p.vec, patch, v);
+                    store_as(p.u, p.out_type, at, p.ldo, live, valid, p.vec, patch, w);
                 }
 #pragma unroll
-                for (int i = 0; i < 64; ++i) gate[i] = silu(gate[i]) * up[i];
-                store_as(p.out[0], p.out_type, at, valid, p.vec, gate);
-            } else {
-                store_as(c.z ? p.out[1] : p.out[0], p.out_type, at, valid, p.vec, v);
+                for (int i = 0; i < COLS; ++i) v[i] = silu(v[i]) * w[i];
             }
+            store_as(c.z ? p.out[1] : p.out[0], p.out_type, at, p.ldo, live, valid, p.vec, patch, v);
         }
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -311,15 +347,9 @@ template <bool GATED> __device__ __forceinline__ void few_store(const FewPlan& p
     store_one(p.out, p.out_type, at, a);
 }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-    uint32_t there;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to(addr, rank)) : "memory");
     return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void load8_any(const FewPlan& p, uint64_t at, float (&v)[8]) {
     if (p.x_dtype == ZC_BF16) p.x_vec ? load8<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(p.x) + at, v) : load8<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(p.x) + at, v);
@@ -352,7 +382,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_s)), "r"(p.tmem_columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         for (uint32_t k = k0; k < min(k0 + p.prefetch, k1); ++k) {
             const uint32_t seg = k / p.kblocks, kb = k % p.kblocks;
             for (uint32_t i = 0; i < MATS; ++i) {
@@ -375,15 +405,17 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     const uint32_t b_bytes = fused ? 0 : p.n * 128, xtiles = p.n > 128 ? 2 : 1;      // token rows of a stage; scale tiles of the tokens
     const uint32_t sf_off = MATS * A_BYTES + b_bytes;
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
+        if (elect_one()) {
+            // slot, its round, segment and block are counted, not divided for: a division a stage is what the loop would wait for
+            uint32_t it = 0, slot = 0, round = 0, seg = k0 / p.kblocks, kb = k0 % p.kblocks;
+            const bool two = xtiles == 2 && p.tokens > 128;
             bool ok = true;
             for (uint32_t k = k0; k < k1; ++k, ++it) {
-                const uint32_t slot = it % p.stages, a = ring + slot * p.stage, seg = k / p.kblocks, kb = k % p.kblocks;
-                if (it >= p.stages && !mbar_wait(&empty[slot], (it / p.stages - 1) & 1, abort_flag, status)) { ok = false; break; }
+                const uint32_t a = ring + slot * p.stage;
+                if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
                 const uint32_t atoms = MX4 ? min(2u, p.ktiles - kb * 2) : 0;
-                const bool two = xtiles == 2 && p.tokens > 128;
                 mbar_expect(&full[slot], MATS * A_BYTES + b_bytes + atoms * 512 * (MATS + (fused ? 0 : two ? 2 : 1)));
+#pragma unroll
                 for (uint32_t i = 0; i < MATS; ++i) {
                     if constexpr (A_MN) {
                         tma_load_2d(a, &maps.a[seg], &full[slot], m0, kb * 64);
@@ -400,6 +432,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                         if (two) bulk_load(a + sf_off + MATS * 1024 + 1024, p.sfx + (uint64_t(p.ktiles) + kb * 2) * 512, atoms * 512, &full[slot]);
                     }
                 }
+                if (++slot == p.stages) { slot = 0; ++round; }
+                if (++kb == p.kblocks) { kb = 0; ++seg; }
             }
             if (!ok)
                 for (uint32_t f = it > p.stages ? it - p.stages : 0; f < it; ++f)
@@ -407,35 +441,48 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status);
-            uint32_t it = 0, more = 0;
-            for (uint32_t k = k0; ok && k < k1; ++k, ++it) {
-                const uint32_t slot = it % p.stages, a = ring + slot * p.stage, kb = k % p.kblocks;
-                if (!mbar_wait(&full[slot], (it / p.stages) & 1, abort_flag, status)) { ok = false; break; }
+            uint32_t slot = 0, phase = 0, kb = k0 % p.kblocks, more = 0;
+            uint32_t quantised = ring + p.resident;
+            for (uint32_t k = k0; ok && k < k1; ++k) {
+                const uint32_t a = ring + slot * p.stage;
+                if (!mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t b = fused ? ring + p.resident + it * (p.n * 128 + 1024) : a + MATS * A_BYTES;
+                const uint32_t b = fused ? quantised : a + MATS * A_BYTES;
                 const uint32_t sfb = fused ? b + p.n * 128 : a + sf_off + MATS * 1024;
                 const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4, sf = tmem + p.sf_column + slot * p.sf_columns;
-                const uint64_t db = desc_at(DESC_K_MAJOR, b);
+                const uint64_t db = desc_at(DESC_K_MAJOR, b), da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a);
                 if constexpr (MX4) {
-                    for (uint32_t j = 0; j < (steps + 1) / 2; ++j) {
-                        for (uint32_t i = 0; i < MATS; ++i) tmem_copy_scales(sf + i * 8 + j * 4, desc_at(DESC_SCALES, a + sf_off + i * 1024 + j * 512));
-                        for (uint32_t i = 0; i < xtiles; ++i) tmem_copy_scales(sf + MATS * 8 + j * 4 * xtiles + i * 4, desc_at(DESC_SCALES, sfb + i * 1024 + j * 512));
+                    const uint64_t dsa = desc_at(DESC_SCALES, a + sf_off), dsb = desc_at(DESC_SCALES, sfb);
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {
+                        if (j * 2 >= steps) break;
+#pragma unroll
+                        for (uint32_t i = 0; i < MATS; ++i) tmem_copy_scales(sf + i * 8 + j * 4, dsa + i * 64 + j * 32);
+                        tmem_copy_scales(sf + MATS * 8 + j * 4 * xtiles, dsb + j * 32);
+                        if (xtiles == 2) tmem_copy_scales(sf + MATS * 8 + j * 8 + 4, dsb + 64 + j * 32);
                     }
                 }
-                for (uint32_t s = 0; s < steps; ++s, more = 1) {
+#pragma unroll
+                for (uint32_t s = 0; s < 4; ++s) {
+                    if (s >= steps) break;
+#pragma unroll
                     for (uint32_t i = 0; i < MATS; ++i) {
-                        const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a + i * A_BYTES);
                         if constexpr (MX4) {
-                            const uint32_t id = (s & 1) * 2;
-                            umma_mx4(tmem + i * p.n, da + s * 2, db + s * 2, p.idesc | id << 29 | id << 4, sf + i * 8 + (s >> 1) * 4, sf + MATS * 8 + (s >> 1) * 4 * xtiles, more);
+                            constexpr uint32_t odd = 2u << 29 | 2u << 4;
+                            umma_mx4(tmem + i * p.n, da + i * (A_BYTES >> 4) + s * 2, db + s * 2, s & 1 ? p.idesc | odd : p.idesc, sf + i * 8 + (s >> 1) * 4,
+                                     sf + MATS * 8 + (s >> 1) * 4 * xtiles, more);
                         } else {
-                            umma_f16(tmem + i * p.n, da + s * (A_MN ? 128 : 2), db + s * 2, p.idesc, more);
+                            umma_f16(tmem + i * p.n, da + i * (A_BYTES >> 4) + s * (A_MN ? 128 : 2), db + s * 2, p.idesc, more);
                         }
                     }
+                    more = 1;
                 }
                 umma_commit(&empty[slot]);
+                if (++slot == p.stages) { slot = 0; phase ^= 1; }
+                if (++kb == p.kblocks) kb = 0;
+                quantised += p.n * 128 + 1024;
             }
             if (ok) umma_commit(&acc_full);
             else {
@@ -566,17 +613,25 @@ bool make_map(CUtensorMap& m, const void* base, bool bytes, uint64_t inner, uint
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 bool map_codes(CUtensorMap& m, const void* codes, uint32_t rows, uint32_t cols, uint32_t box) { return make_map(m, codes, true, cols / 2, rows, cols / 2, box); }
-// A 16-bit operand [rows, cols]: K along its rows (boxes of 64 k x 128 rows, or of so many), or across them (boxes of 64 columns x 64 k).
-bool map_rows(CUtensorMap& m, const void* p, uint32_t rows, uint32_t cols, uint64_t ld, bool k_across, uint32_t box = TILE_M) {
-    return make_map(m, p, false, cols, rows, ld * 2, k_across ? 64 : box);
+// Scale tiles as rows of 512 bytes, two a box.
+bool map_scales(CUtensorMap& m, const void* scales, uint32_t rows, uint32_t cols) {
+    const Encode encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {128, mx4_scale_bytes(rows, cols) / 512}, strides[1] = {512};
+    const cuuint32_t box[2] = {128, 2}, elem[2] = {1, 1};
+    return encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// A 16-bit operand [rows, cols]: K along its rows (boxes of 64 k x `box` rows), or across them (boxes of 64 columns x 64 k).
+bool map_rows(CUtensorMap& m, const void* p, uint32_t rows, uint32_t cols, uint64_t ld, uint32_t box) { return make_map(m, p, false, cols, rows, ld * 2, box); }
+constexpr uint32_t ACROSS = 64;
 
-// Instruction descriptors. Both: N / 8 from bit 17, M / 16 from bit 24.
-uint32_t idesc_f16(int dtype, bool a_mn, bool b_mn, uint32_t n = TILE_N) {      // FP32 accumulators; operand types; which operand has M / N along its rows
+// Instruction descriptors. Both: N / 8 from bit 17, M / 16 from bit 24 (M = 128 of one CTA, 256 of a pair).
+uint32_t idesc_f16(int dtype, bool a_mn, bool b_mn, uint32_t m, uint32_t n) {      // FP32 accumulators; operand types; which operand has M / N along its rows
     const uint32_t t = dtype == ZC_BF16 ? 1 : 0;
-    return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | ((n / 8) << 17) | ((TILE_M / 16) << 24);
+    return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | ((n / 8) << 17) | ((m / 16) << 24);
 }
-uint32_t idesc_mx4(uint32_t n = TILE_N) { return (1u << 7) | (1u << 10) | ((n / 8) << 17) | (1u << 23) | ((TILE_M / 16) << 24); }      // e2m1 both, e8m0 scales
+uint32_t idesc_mx4(uint32_t m, uint32_t n) { return (1u << 7) | (1u << 10) | ((n / 8) << 17) | (1u << 23) | ((m / 16) << 24); }      // e2m1 both, e8m0 scales
 
 struct Device { int index = -1; uint32_t sms = 0; };
 int current_device(Device& d) {
@@ -604,22 +659,29 @@ struct Configured {
     }
 };
 
-template <bool MX4, bool A_MN, bool B_MN, bool GATED> int launch_tiles(const TileMaps& maps, TilePlan& p, cudaStream_t s) {
-    Device d;
-    int rc = current_device(d);
-    if (rc != ZC_OK) return rc;
+template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(const TileMaps& maps, TilePlan& p, const Device& d, cudaStream_t s) {
     static Configured configured;
-    auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED>;
-    if ((rc = configured.once(kernel, d.index, TileSmem<MX4>::bytes)) != ZC_OK) return rc;
-    constexpr uint32_t width = GATED ? TILE_N / 2 : TILE_N;
-    p.mtiles = (p.M + TILE_M - 1) / TILE_M;
+    auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED, N>;
+    constexpr uint32_t smem = TileSmem<MX4, N>::bytes;
+    const int rc = configured.once(kernel, d.index, smem);
+    if (rc != ZC_OK) return rc;
+    p.vec = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && (!p.out[1] || rows16(p.out[1], p.ldo, dtype_bytes(p.out_type)));
+    const uint32_t pairs = d.sms / 2;
+    return launched(launch_after(kernel, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), THREADS, smem, 2, s, maps, p), "dense product");
+}
+
+// Tiles of `width` output columns; the number of them, or 0 where there are too many.
+uint32_t set_tiles(TilePlan& p, uint32_t width) {
+    p.mtiles = uint32_t((uint64_t(p.M) + 2 * TILE_M - 1) / (2 * TILE_M));
     p.ntiles = (p.N + width - 1) / width;
     const uint64_t tiles = uint64_t(p.mtiles) * p.ntiles * p.outs;
-    if (tiles > 0x7fffffffu) return fail(nullptr, ZC_EINVAL, "too many output tiles");
-    p.tiles = uint32_t(tiles);
-    p.vec = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && (!p.out[1] || rows16(p.out[1], p.ldo, dtype_bytes(p.out_type)));
-    return launched(launch_after(kernel, dim3(p.tiles < d.sms ? p.tiles : d.sms), THREADS, TileSmem<MX4>::bytes, 1, s, maps, p), "dense product");
+    return p.tiles = tiles > 0x7fffffffu ? 0 : uint32_t(tiles);
 }
+// Whether 128 columns a tile: where 256 leave half of the pairs without one.
+bool narrow_tiles(TilePlan& p, const Device& d, uint32_t per_output) {
+    return set_tiles(p, 256 / per_output) <= d.sms / 4;
+}
+int too_many() { return fail(nullptr, ZC_EINVAL, "too many output tiles"); }
 
 template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block) {
     p.kblocks = (k + block - 1) / block;
@@ -699,7 +761,7 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
             p.sfw[i] = static_cast<const uint8_t*>(w[i].scales);
         }
         if (!p.resident && !map_codes(maps.b[0], x_codes, tokens, cols, p.n)) return no_maps();
-        p.idesc = idesc_mx4(p.n);
+        p.idesc = idesc_mx4(TILE_M, p.n);
         p.ktiles = (cols + 127) / 128;
         p.sfx = static_cast<const uint8_t*>(x_scales);
         p.x = x; p.x_ld = x_ld; p.x_dtype = x_dtype; p.cols = cols;
@@ -709,17 +771,19 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     }
     if (x && (rc = launch_mx4_quantize(x, x_dtype, tokens, cols, x_ld, x_codes, x_scales, s)) != ZC_OK) return rc;
     TilePlan p{};
-    if (!map_codes(maps.a[0], x_codes, tokens, cols, TILE_M)) return no_maps();
-    for (int i = 0; i < mats; ++i)
-        if (!map_codes(maps.b[i], w[i].codes, rows, cols, TILE_M)) return no_maps();
     p.M = tokens; p.N = rows; p.segs = 1; p.outs = 1;
     set_k(p, cols, 256);
-    p.idesc = idesc_mx4();
-    p.ktiles = (cols + 127) / 128; p.brows = rows;
-    p.sfa = static_cast<const uint8_t*>(x_scales);
-    for (int i = 0; i < mats; ++i) p.sfb[i] = static_cast<const uint8_t*>(w[i].scales);
+    p.ktiles = (cols + 127) / 128;
     p.out[0] = out; p.ldo = out_ld; p.out_type = out_dtype;
-    return mats == 2 ? launch_tiles<true, false, false, true>(maps, p, s) : launch_tiles<true, false, false, false>(maps, p, s);
+    const bool narrow = mats == 1 && narrow_tiles(p, d, 1);        // gated: 64 rows each of gate and up would share a scale tile
+    const uint32_t n = narrow ? 128 : 256;
+    if (!set_tiles(p, n / mats)) return too_many();
+    p.idesc = idesc_mx4(256, n);
+    if (!map_codes(maps.a[0], x_codes, tokens, cols, TILE_M) || !map_scales(maps.sfa, x_scales, tokens, cols)) return no_maps();
+    for (int i = 0; i < mats; ++i)
+        if (!map_codes(maps.b[i], w[i].codes, rows, cols, n / 2) || !map_scales(maps.sfb[i], w[i].scales, rows, cols)) return no_maps();
+    if (mats == 2) return launch_tiles<true, false, false, true, 256>(maps, p, d, s);
+    return narrow ? launch_tiles<true, false, false, false, 128>(maps, p, d, s) : launch_tiles<true, false, false, false, 256>(maps, p, d, s);
 }
 
 int check_gated(const char* who, int dtype, uint32_t hidden, uint32_t ffn) {
@@ -764,28 +828,31 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
         for (const Span& v : in) if (overlap(to[i], v)) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
         for (int j = 0; j < i; ++j) if (overlap(to[i], to[j])) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
     }
+    Device d;
+    if ((rc = current_device(d)) != ZC_OK) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     TileMaps maps{};
     if (tokens <= FEW_TOKENS) {
-        Device d;
-        if ((rc = current_device(d)) != ZC_OK) return rc;
         FewPlan p{};
         p.M = ffn; p.tokens = tokens; p.segs = 1;
         set_k(p, hidden, 64);
         plan_few(p, false, 2, false, d.sms);
-        if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, false) || !map_rows(maps.a[1], up, ffn, hidden, hidden, false) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, false, p.n))
+        if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, TILE_M) || !map_rows(maps.a[1], up, ffn, hidden, hidden, TILE_M) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, p.n))
             return no_maps();
-        p.idesc = idesc_f16(dtype, false, false, p.n);
+        p.idesc = idesc_f16(dtype, false, false, TILE_M, p.n);
         p.out = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
-        return launch_few<false, false, 2>(maps, p, d, static_cast<cudaStream_t>(stream));
+        return launch_few<false, false, 2>(maps, p, d, s);
     }
     TilePlan p{};
-    if (!map_rows(maps.a[0], x, tokens, hidden, x_ld, false) || !map_rows(maps.b[0], gate, ffn, hidden, hidden, false) || !map_rows(maps.b[1], up, ffn, hidden, hidden, false))
-        return no_maps();
     p.M = tokens; p.N = ffn; p.segs = 1; p.outs = 1;
     set_k(p, hidden, 64);
-    p.idesc = idesc_f16(dtype, false, false);
     p.out[0] = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
-    return launch_tiles<false, false, false, true>(maps, p, static_cast<cudaStream_t>(stream));
+    const bool narrow = narrow_tiles(p, d, 2);
+    const uint32_t n = narrow ? 128 : 256;
+    if (!set_tiles(p, n / 2)) return too_many();
+    p.idesc = idesc_f16(dtype, false, false, 256, n);
+    if (!map_rows(maps.a[0], x, tokens, hidden, x_ld, TILE_M) || !map_rows(maps.b[0], gate, ffn, hidden, hidden, n / 2) || !map_rows(maps.b[1], up, ffn, hidden, hidden, n / 2)) return no_maps();
+    return narrow ? launch_tiles<false, false, false, true, 128>(maps, p, d, s) : launch_tiles<false, false, false, true, 256>(maps, p, d, s);
 }
 
 int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_ld, const void* gate, const void* up, const void* g, const void* u, int dtype, uint32_t tokens,
@@ -823,39 +890,45 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     };
     rc = launched(dtype == ZC_BF16 ? gradient(gated_gradient_kernel<__nv_bfloat16>, __nv_bfloat16()) : gradient(gated_gradient_kernel<__half>, __half()), "gated gradient");
     if (rc != ZC_OK) return rc;
-    if (dx && tokens <= FEW_TOKENS) {
-        Device d;
-        if ((rc = current_device(d)) != ZC_OK) return rc;
+    Device d;
+    if ((rc = current_device(d)) != ZC_OK) return rc;
+    if (dx) {
         TileMaps maps{};
-        FewPlan p{};
-        p.M = hidden; p.tokens = tokens; p.segs = 2;
-        set_k(p, ffn, 64);
-        plan_few(p, false, 1, false, d.sms);
-        if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, true) || !map_rows(maps.a[1], up, ffn, hidden, hidden, true) ||
-            !map_rows(maps.b[0], dg, tokens, ffn, ffn, false, p.n) || !map_rows(maps.b[1], du, tokens, ffn, ffn, false, p.n)) return no_maps();
-        p.idesc = idesc_f16(dtype, true, false, p.n);
-        p.out = dx; p.ldo = hidden; p.out_type = dtype;
-        if ((rc = launch_few<false, true, 1>(maps, p, d, s)) != ZC_OK) return rc;
-    } else if (dx) {
-        TileMaps maps{};
-        TilePlan p{};
-        if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, false) || !map_rows(maps.a[1], du, tokens, ffn, ffn, false) ||
-            !map_rows(maps.b[0], gate, ffn, hidden, hidden, true) || !map_rows(maps.b[1], up, ffn, hidden, hidden, true)) return no_maps();
-        p.M = tokens; p.N = hidden; p.segs = 2; p.outs = 1;
-        set_k(p, ffn, 64);
-        p.idesc = idesc_f16(dtype, false, true);
-        p.out[0] = dx; p.ldo = hidden; p.out_type = dtype;
-        if ((rc = launch_tiles<false, false, true, false>(maps, p, s)) != ZC_OK) return rc;
+        if (tokens <= FEW_TOKENS) {
+            FewPlan p{};
+            p.M = hidden; p.tokens = tokens; p.segs = 2;
+            set_k(p, ffn, 64);
+            plan_few(p, false, 1, false, d.sms);
+            if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, ACROSS) || !map_rows(maps.a[1], up, ffn, hidden, hidden, ACROSS) ||
+                !map_rows(maps.b[0], dg, tokens, ffn, ffn, p.n) || !map_rows(maps.b[1], du, tokens, ffn, ffn, p.n)) return no_maps();
+            p.idesc = idesc_f16(dtype, true, false, TILE_M, p.n);
+            p.out = dx; p.ldo = hidden; p.out_type = dtype;
+            rc = launch_few<false, true, 1>(maps, p, d, s);
+        } else {
+            TilePlan p{};
+            p.M = tokens; p.N = hidden; p.segs = 2; p.outs = 1;
+            set_k(p, ffn, 64);
+            p.out[0] = dx; p.ldo = hidden; p.out_type = dtype;
+            const bool narrow = narrow_tiles(p, d, 1);
+            if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
+            p.idesc = idesc_f16(dtype, false, true, 256, narrow ? 128 : 256);
+            if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, TILE_M) || !map_rows(maps.a[1], du, tokens, ffn, ffn, TILE_M) ||
+                !map_rows(maps.b[0], gate, ffn, hidden, hidden, ACROSS) || !map_rows(maps.b[1], up, ffn, hidden, hidden, ACROSS)) return no_maps();
+            rc = narrow ? launch_tiles<false, false, true, false, 128>(maps, p, d, s) : launch_tiles<false, false, true, false, 256>(maps, p, d, s);
+        }
+        if (rc != ZC_OK) return rc;
     }
     if (dgate) {
         TileMaps maps{};
         TilePlan p{};
-        if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, true) || !map_rows(maps.a[1], du, tokens, ffn, ffn, true) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, true)) return no_maps();
         p.M = ffn; p.N = hidden; p.segs = 1; p.outs = 2;
         set_k(p, tokens, 64);
-        p.idesc = idesc_f16(dtype, true, true);
         p.out[0] = dgate; p.out[1] = dup; p.ldo = hidden; p.out_type = dtype;
-        rc = launch_tiles<false, true, true, false>(maps, p, s);
+        const bool narrow = narrow_tiles(p, d, 1);
+        if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
+        p.idesc = idesc_f16(dtype, true, true, 256, narrow ? 128 : 256);
+        if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, ACROSS) || !map_rows(maps.a[1], du, tokens, ffn, ffn, ACROSS) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, ACROSS)) return no_maps();
+        rc = narrow ? launch_tiles<false, true, true, false, 128>(maps, p, d, s) : launch_tiles<false, true, true, false, 256>(maps, p, d, s);
     }
     return rc;
 }
