@@ -52,9 +52,9 @@ __device__ uint32_t ffn_status_word;     // the device's status word of these op
 constexpr uint32_t TILE_M = 128, THREADS = 320;           // rows of a CTA
 constexpr uint32_t A_BYTES = TILE_M * 128;
 constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory columns of a stage's scales: A 2 x 4, B 2 x 8 at most
-constexpr uint32_t PATCH = 9;                              // floats of a row of the patch that a warp turns where rows are not aligned
+constexpr uint32_t PATCH = 17, PATCH_BYTES = 4096;         // a warp's shared memory of the epilogue, and the floats of a row where it turns rows in it
 
-struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2]; };
+struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
 struct TilePlan {
     uint32_t M, N;                      // rows and columns of an output (gated: N = ffn)
@@ -67,7 +67,7 @@ struct TilePlan {
     uint64_t ldo;
     void *g, *u;                        // gated: where the two products go as well, or null
     int out_type;
-    bool vec;                           // the output's rows are 16-byte aligned
+    bool aligned;                       // the output's rows are 16-byte aligned: o[] are views of out[0], and of out[1], or of g and u
 };
 
 struct Tile { uint32_t z, m0, n0; };
@@ -79,52 +79,58 @@ __device__ __forceinline__ Tile tile_at(const TilePlan& p, uint32_t t, uint32_t 
     return {z, (band * 8 + j % rows) * 2 * TILE_M, j / rows * width};
 }
 
-// A warp's 32 rows (one a lane) of NC columns: `live`, the lane's row exists; `valid` leading columns do. Rows that are 16-byte aligned are
-// stored by their lanes, 16 bytes at a time. Others are turned eight columns at a time through a patch of shared memory, so that eight
-// lanes store consecutive columns (a lane's own row, value by value, would touch 32 sectors a store: 45 -> 25 us for 257 x 10007).
-template <typename T, int NC> __device__ __forceinline__ void store_rows(T* to, uint64_t ld, bool live, uint32_t valid, bool vec, float* patch, const float (&v)[NC]) {
-    constexpr int PER = 16 / sizeof(T);
-    if (vec) {
-        if (!live) return;
+// A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on; rows past `rows` and columns past `cols` are left out. Rows that
+// are 16-byte aligned leave by TMA: 128 (or 64) bytes of each through shared memory, swizzled so that neither side meets a bank twice.
+// Stored by the lanes, 16 bytes of a row each, they took 6,200 clocks a tile, and the waits of the copying and the issuing
+// thread queued behind them. Rows that are not aligned are turned sixteen columns at a time through the same memory, so that
+// sixteen lanes store consecutive columns (257 x 10007: 45 -> 23 us against values stored by the rows' own lanes).
+template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (row >= p.M) return;
+    if (p.aligned) {
+        constexpr int GROUP = NC * int(sizeof(T)) < 128 ? NC : 128 / int(sizeof(T)), CHUNK = 16 / sizeof(T), BYTES = GROUP * sizeof(T);
 #pragma unroll
-        for (int c = 0; c < NC; c += PER) {
-            if (c + PER <= valid) {
-                alignas(16) T w[PER];
+        for (int c = 0; c < NC; c += GROUP) {
+            if (col + c >= p.N) break;
+            if (lane == 0) tma_store_read();
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < PER; ++j) w[j] = from_f32<T>(v[c + j]);
-                *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(w);
-            } else {
+            for (int j = 0; j < GROUP / CHUNK; ++j) {
+                alignas(16) T w[CHUNK];
 #pragma unroll
-                for (int j = 0; j < PER; ++j)
-                    if (c + j < valid) to[c + j] = from_f32<T>(v[c + j]);
+                for (int k = 0; k < CHUNK; ++k) w[k] = from_f32<T>(v[c + j * CHUNK + k]);
+                const uint32_t turn = BYTES == 128 ? lane & 7 : (lane >> 1) & 3;
+                *reinterpret_cast<uint4*>(patch + lane * BYTES + ((j ^ turn) << 4)) = *reinterpret_cast<const uint4*>(w);
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map, smem_addr(patch), col + c, row);
         }
         return;
     }
-    const uint32_t lane = threadIdx.x & 31, rows = __popc(__ballot_sync(0xffffffffu, live));
-    T* const first = to - lane * ld;
+    float* const turned = reinterpret_cast<float*>(patch);
+    const uint32_t rows = min(32u, p.M - row);
 #pragma unroll
-    for (int c = 0; c < NC; c += 8) {
+    for (int c = 0; c < NC; c += 16) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) patch[lane * PATCH + j] = v[c + j];
+        for (int j = 0; j < 16; ++j) turned[lane * PATCH + j] = v[c + j];
         __syncwarp();
-        const uint32_t col = c + (lane & 7);
-#pragma unroll
-        for (uint32_t r = lane >> 3; r < 32; r += 4)
-            if (r < rows && col < valid) first[r * ld + col] = from_f32<T>(patch[r * PATCH + (lane & 7)]);
+        const uint32_t at = col + c + (lane & 15);
+        if (at < p.N)
+            for (uint32_t r = lane >> 4; r < rows; r += 2) out[uint64_t(row + r) * p.ldo + at] = from_f32<T>(turned[r * PATCH + (lane & 15)]);
         __syncwarp();
     }
 }
-template <int NC> __device__ __forceinline__ void store_as(void* out, int type, uint64_t at, uint64_t ld, bool live, uint32_t valid, bool vec, float* patch, const float (&v)[NC]) {
-    if (type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out) + at, ld, live, valid, vec, patch, v);
-    else if (type == ZC_F16) store_rows(static_cast<__half*>(out) + at, ld, live, valid, vec, patch, v);
-    else store_rows(static_cast<float*>(out) + at, ld, live, valid, vec, patch, v);
+template <int NC> __device__ __forceinline__ void store_as(void* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    if (p.out_type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
+    else if (p.out_type == ZC_F16) store_rows(static_cast<__half*>(out), map, p, row, col, patch, v);
+    else if constexpr (NC >= 64) store_rows(static_cast<float*>(out), map, p, row, col, patch, v);      // (16-bit operands have 16-bit results)
 }
 __device__ __forceinline__ float silu(float v) { return __fdiv_rn(v, 1.0f + expf(-v)); }
 
 template <bool MX4, int N> struct TileSmem {
-    static constexpr uint32_t b = N / 2 * 128, stage = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), stages = 6, patches = 8 * 32 * PATCH * 4;
-    static constexpr uint32_t bytes = stages * stage + patches + 1024;
+    static constexpr uint32_t b = N / 2 * 128, stage = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0);
+    static constexpr uint32_t stages = MX4 && N == 256 ? 5 : 6, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
 };
 
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     } else {
         constexpr int COLS = WIDTH / 2;                                 // output columns of a warp
         const uint32_t half = (warp - 2) >> 2, quarter = warp & 3;      // which columns; the 32 lanes of tensor memory a warp can read
-        float* const patch = reinterpret_cast<float*>(raw + (ring - smem_addr(raw)) + STAGES * STAGE) + (warp - 2) * 32 * PATCH;
+        uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * PATCH_BYTES;
         uint32_t n = 0;
         for (uint32_t t = pair; t < p.tiles; t += pairs, ++n) {
             const Tile c = tile_at(p, t, WIDTH);
@@ -275,21 +281,18 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_at(map_to(smem_addr(&acc_empty[buf]), 0));
-            const uint32_t row = c.m0 + rank * TILE_M + quarter * 32 + lane, col = c.n0 + half * COLS;
-            if (col >= p.N) continue;
-            const uint64_t at = uint64_t(row) * p.ldo + col;
-            const uint32_t valid = p.N - col;
-            const bool live = row < p.M;
+            const uint32_t row = c.m0 + rank * TILE_M + quarter * 32, col = c.n0 + half * COLS;
             if constexpr (GATED) {
                 if (p.g) {
-                    store_as(p.g, p.out_type, at, p.ldo, live, valid, p.vec, patch, v);
-                    store_as(p.u, p.out_type, at, p.ldo, live, valid, p.vec, patch, w);
+                    store_as(p.g, &maps.o[1], p, row, col, patch, v);
+                    store_as(p.u, &maps.o[2], p, row, col, patch, w);
                 }
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = silu(v[i]) * w[i];
             }
-            store_as(c.z ? p.out[1] : p.out[0], p.out_type, at, p.ldo, live, valid, p.vec, patch, v);
+            store_as(c.z ? p.out[1] : p.out[0], &maps.o[c.z], p, row, col, patch, v);
         }
+        if (lane == 0) tma_store_done();
         __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -647,6 +650,18 @@ int current_device(Device& d) {
     return ZC_OK;
 }
 
+int no_maps() { return fail(nullptr, ZC_EEXEC, "the driver did not encode a tensor map"); }
+// The output in boxes of 32 rows x 128 bytes, or of what a warp has of a row.
+bool map_output(CUtensorMap& m, void* out, const TilePlan& p, uint32_t columns) {
+    const Encode encode = tensor_map_encoder();
+    if (!encode) return false;
+    const uint32_t elem_bytes = uint32_t(dtype_bytes(p.out_type)), most = 128 / elem_bytes;
+    const cuuint64_t dims[2] = {p.N, p.M}, strides[1] = {p.ldo * elem_bytes};
+    const cuuint32_t box[2] = {columns < most ? columns : most, 32}, elem[2] = {1, 1};
+    return encode(&m, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, out, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  columns < most ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The opt-in to large shared memory of one kernel, once per device.
 struct Configured {
     std::atomic<bool> done[MAX_DEVICES] = {};
@@ -659,13 +674,16 @@ struct Configured {
     }
 };
 
-template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(const TileMaps& maps, TilePlan& p, const Device& d, cudaStream_t s) {
+template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(TileMaps& maps, TilePlan& p, const Device& d, cudaStream_t s) {
     static Configured configured;
     auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED, N>;
     constexpr uint32_t smem = TileSmem<MX4, N>::bytes;
     const int rc = configured.once(kernel, d.index, smem);
     if (rc != ZC_OK) return rc;
-    p.vec = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && (!p.out[1] || rows16(p.out[1], p.ldo, dtype_bytes(p.out_type)));
+    void* const to[3] = {p.out[0], p.g ? p.g : p.out[1], p.u};
+    p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type));        // (the others are contiguous and aligned wherever they are given)
+    for (int i = 0; i < 3 && p.aligned; ++i)
+        if (to[i] && !map_output(maps.o[i], to[i], p, GATED ? N / 4 : N / 2)) return no_maps();
     const uint32_t pairs = d.sms / 2;
     return launched(launch_after(kernel, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), THREADS, smem, 2, s, maps, p), "dense product");
 }
@@ -726,7 +744,6 @@ template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, Fe
     return launched(launch_after(kernel, dim3((p.M + TILE_M - 1) / TILE_M * p.splits), FEW_THREADS, p.smem, p.splits, s, maps, p), "dense product of few tokens");
 }
 
-int no_maps() { return fail(nullptr, ZC_EEXEC, "the driver did not encode a tensor map"); }
 
 struct Mx4Arg { const void *codes, *scales; };
 
