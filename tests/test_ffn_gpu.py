@@ -168,17 +168,19 @@ def test_linear_scales_of_every_size(ffn, tokens):
     close(ffn.mx4_linear(qx, qw, torch.float32), ref.of(qx) @ ref.of(qw).T, sums(ref.of(qx), ref.of(qw), 64))
 
 
-def test_outputs_of_the_caller_keep_what_lies_around_them(ffn):
+@pytest.mark.parametrize("tokens,rows", [(1, 90), (35, 90), (70, 90), (70, 96), (300, 700), (35, 2000)])
+def test_outputs_of_the_caller_keep_what_lies_around_them(ffn, tokens, rows):
     """Views as output: row strides of every alignment, the rows and columns around the result untouched."""
-    x, w = ffn.mx4_quantize(randn((70, 128), 1)), ffn.mx4_quantize(randn((90, 128), 2))
-    want = ffn.mx4_linear(x, w, torch.float32)
+    x, w, v = ffn.mx4_quantize(randn((tokens, 1056), 1)), ffn.mx4_quantize(randn((rows, 1056), 2)), ffn.mx4_quantize(randn((rows, 1056), 3))
+    want, gated = ffn.mx4_linear(x, w, torch.float32), ffn.mx4_gated(x, w, v, torch.float32)
     for dtype in TYPES:
-        for left, right in ((0, 1), (1, 2), (8, 6), (16, 22)):
-            big = torch.full((74, 90 + left + right), 7.0, dtype=dtype, device="cuda")
-            out = big[2:72, left:left + 90]
+        for left, right in ((0, 1), (1, 2), (8, 6), (16, 22), (8, 0), (0, 8)):
+            big = torch.full((tokens + 4, rows + left + right), 7.0, dtype=dtype, device="cuda")
+            out = big[2:tokens + 2, left:left + rows]
             assert ffn.mx4_linear(x, w, out=out) is out
             assert torch.equal(out, want.to(dtype))
-            big[2:72, left:left + 90] = 7.0
+            assert torch.equal(ffn.mx4_gated(x, w, v, out=out), gated.to(dtype))
+            out.fill_(7.0)
             assert bool((big == 7.0).all())
 
 

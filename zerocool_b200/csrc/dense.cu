@@ -67,7 +67,7 @@ struct TilePlan {
     uint64_t ldo;
     void *g, *u;                        // gated: where the two products go as well, or null
     int out_type;
-    bool aligned;                       // the output's rows are 16-byte aligned: o[] are views of out[0], and of out[1], or of g and u
+    bool aligned;                       // the output's rows start and end on 16 bytes: o[] are views of out[0], and of out[1], or of g and u
 };
 
 struct Tile { uint32_t z, m0, n0; };
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     const CUtensorMap* const mb = &maps.b[GATED ? rank : s];
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++it) {
                         const uint32_t a = ring + slot * STAGE, b = a + A_BYTES;
-                        if (round && !mbar_wait_cluster(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
+                        if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
                         const uint32_t bar = map_to(smem_addr(&full[slot]), 0);             // the leader counts the bytes of both
                         if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
                         if constexpr (A_MN) {
@@ -213,20 +213,22 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
             uint32_t n = 0, slot = 0, phase = 0;
-            bool ok = true;
+            bool ok = true, ready = mbar_test(&full[0], 0);      // a stage ahead: the answer arrives while the products before it are issued
             for (uint32_t t = pair; ok && t < p.tiles; t += pairs, ++n) {
                 const uint32_t buf = n % ACC, acc = tmem + buf * N;
-                if (n >= ACC && !mbar_wait_cluster(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
+                if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t more = 0;
                 for (uint32_t s = 0; ok && s < p.segs; ++s) {
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES;
-                        if (!mbar_wait_cluster(&full[slot], phase, abort_flag, status)) { ok = false; break; }
+                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES, now = slot;
+                        if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
+                        ready = mbar_test(&full[slot], phase);
                         const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
                         const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4;
-                        const uint32_t sf = tmem + SF_COLUMN + slot * SF_COLUMNS;
+                        const uint32_t sf = tmem + SF_COLUMN + now * SF_COLUMNS;
                         if constexpr (MX4) {
                             // 128 k of scales: four columns for A's rows, four or eight for B's
                             const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
@@ -249,15 +251,14 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                             }
                             more = 1;
                         }
-                        umma_commit_pair(&empty[slot]);
-                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
+                        umma_commit_pair(&empty[now]);
                     }
                 }
                 if (ok) umma_commit_pair(&acc_full[buf]);
             }
             if (abort_s) {       // products in flight read shared memory and write tensor memory: they end first
                 umma_commit_pair(&drain);
-                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try_cluster(&drain, 0); ++i) {}
+                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
             }
         }
         __syncwarp();
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         for (uint32_t t = pair; t < p.tiles; t += pairs, ++n) {
             const Tile c = tile_at(p, t, WIDTH);
             const uint32_t buf = n % ACC, acc = tmem + buf * N + (quarter << 21);
-            if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[buf], (n / ACC) & 1, abort_flag, status))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (n / ACC) & 1, abort_flag, status))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float v[COLS], w[GATED ? COLS : 1];
 #pragma unroll
@@ -309,13 +310,15 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // one tile of 128 weight rows (of gate and of up) and one run of blocks of K; the CTAs of a cluster share a tile's K and add their partial
 // sums through distributed shared memory, in the order of their ranks. The lanes of the epilogue hold consecutive output columns of
 // a token, so plain stores are coalesced whatever the row stride.
-// x given plain: every CTA quantises its own part of the tokens' K into shared memory (the epilogue warps, while the weights arrive),
-// in the swizzle TMA would have written. The kernel before may still run while this one starts (programmatic launch): until it has
+// One or two plain tokens: every CTA quantises its own part of their K into shared memory (the epilogue warps, while the weights arrive),
+// in the swizzle TMA would have written (more are quantised by a launch of their own). The kernel before may still run while this one starts (programmatic launch): until it has
 // ended nothing is read but into L2, where a later write of it would arrive too.
 constexpr uint32_t FEW_THREADS = 192, FEW_STAGES = 8;
-constexpr uint32_t FEW_TOKENS = 128;
+// 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
+constexpr uint32_t FEW_TOKENS = 64;
 constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_SMEM_MAX = 226 * 1024;      // what a ring may take (two CTAs an SM); the most a CTA may have
-constexpr uint32_t FEW_PLAIN_TOKENS = 32, FEW_PLAIN_BYTES = 32 * 1024;    // x is quantised inside up to these
+// x is quantised inside up to these: MX4 8192 x 4096, 1 / 2 / 4 / 8 tokens 6.4 / 7.2 / 8.7 / 11.3 us, by a launch of its own 8.1 / 8.2 / 8.2 / 8.5.
+constexpr uint32_t FEW_PLAIN_TOKENS = 2, FEW_PLAIN_BYTES = 32 * 1024;
 constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
 
 struct FewPlan {
@@ -331,7 +334,7 @@ struct FewPlan {
     const void* x;
     uint64_t x_ld;
     uint32_t x_dtype, cols;
-    bool x_vec;
+    bool x_vec, out_vec;                // rows of x and of the output are aligned
     void *out, *g, *u;
     uint64_t ldo;
     int out_type;
@@ -349,15 +352,60 @@ template <bool GATED> __device__ __forceinline__ void few_store(const FewPlan& p
     }
     store_one(p.out, p.out_type, at, a);
 }
-__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to(addr, rank)) : "memory");
+// Four consecutive columns of a row, `valid` of which exist.
+template <typename T> __device__ __forceinline__ void store_four(void* out, uint64_t at, uint32_t valid, bool vec, const float4& v) {
+    T* const to = static_cast<T*>(out) + at;
+    alignas(16) const T w[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+    if (vec && valid >= 4) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(w);
+        else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(w);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+            if (j < valid) to[j] = w[j];
+    }
+}
+__device__ __forceinline__ void store_four_as(void* out, const FewPlan& p, uint64_t at, uint32_t valid, const float4& v) {
+    if (p.out_type == ZC_BF16) store_four<__nv_bfloat16>(out, at, valid, p.out_vec, v);
+    else if (p.out_type == ZC_F16) store_four<__half>(out, at, valid, p.out_vec, v);
+    else store_four<float>(out, at, valid, p.out_vec, v);
+}
+template <bool GATED> __device__ __forceinline__ void few_store4(const FewPlan& p, uint64_t at, uint32_t valid, float4 a, const float4& b) {
+    if constexpr (GATED) {
+        if (p.g) { store_four_as(p.g, p, at, valid, a); store_four_as(p.u, p, at, valid, b); }
+        a = make_float4(silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w);
+    }
+    store_four_as(p.out, p, at, valid, a);
+}
+__device__ __forceinline__ float4 load_peer(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to(addr, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ void load8_any(const FewPlan& p, uint64_t at, float (&v)[8]) {
-    if (p.x_dtype == ZC_BF16) p.x_vec ? load8<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(p.x) + at, v) : load8<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(p.x) + at, v);
-    else if (p.x_dtype == ZC_F16) p.x_vec ? load8<__half, true>(static_cast<const __half*>(p.x) + at, v) : load8<__half, false>(static_cast<const __half*>(p.x) + at, v);
-    else p.x_vec ? load8<float, true>(static_cast<const float*>(p.x) + at, v) : load8<float, false>(static_cast<const float*>(p.x) + at, v);
+// The tokens' blocks [k0, k0 + blocks) of 256 columns into shared memory: per block n rows of 128 bytes, then two scale tiles. A warp takes a
+// row of a block at a time, eight values a lane (four lanes share a scale). Padding rows stay as they are (their columns are not stored);
+// columns past the last one become zero codes with a zero scale byte. The loop is not unrolled: a launch of a few microseconds waits for
+// its instructions too (gated block of 512 x 2048, one token: 4.1 us, with four rows in flight 4.7).
+template <typename T> __device__ __forceinline__ void quantise_tokens(const FewPlan& p, uint32_t k0, uint32_t blocks, uint8_t* to) {
+    const uint32_t lane = threadIdx.x & 31, size = p.n * 128 + 1024, left = p.cols - k0 * 256;
+    for (uint32_t t = 0; t < p.tokens; ++t) {
+        const T* const row = static_cast<const T*>(p.x) + uint64_t(t) * p.x_ld + uint64_t(k0) * 256;
+#pragma unroll 1
+        for (uint32_t block = (threadIdx.x >> 5) - 2; block < blocks; block += 4) {
+            const uint32_t at = block * 256 + lane * 8;
+            float v[8] = {};
+            if (at < left) p.x_vec ? load8<T, true>(row + at, v) : load8<T, false>(row + at, v);
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t s = mx4_scale(top);
+            uint8_t* const b = to + block * size;
+            *reinterpret_cast<uint32_t*>(b + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = mx4_codes8(v, s);
+            if ((lane & 3) == 0) b[p.n * 128 + (lane >> 4) * 512 + (t & 31) * 16 + (t >> 5) * 4 + ((lane >> 2) & 3)] = uint8_t(s);
+        }
+    }
 }
 
 template <bool MX4, bool A_MN, int MATS>
@@ -448,13 +496,16 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
             bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status);
             uint32_t slot = 0, phase = 0, kb = k0 % p.kblocks, more = 0;
             uint32_t quantised = ring + p.resident;
+            bool ready = mbar_test(&full[0], 0);
             for (uint32_t k = k0; ok && k < k1; ++k) {
-                const uint32_t a = ring + slot * p.stage;
-                if (!mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
+                const uint32_t a = ring + slot * p.stage, now = slot;
+                if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (++slot == p.stages) { slot = 0; phase ^= 1; }
+                ready = mbar_test(&full[slot], phase);
                 const uint32_t b = fused ? quantised : a + MATS * A_BYTES;
                 const uint32_t sfb = fused ? b + p.n * 128 : a + sf_off + MATS * 1024;
-                const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4, sf = tmem + p.sf_column + slot * p.sf_columns;
+                const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4, sf = tmem + p.sf_column + now * p.sf_columns;
                 const uint64_t db = desc_at(DESC_K_MAJOR, b), da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a);
                 if constexpr (MX4) {
                     const uint64_t dsa = desc_at(DESC_SCALES, a + sf_off), dsb = desc_at(DESC_SCALES, sfb);
@@ -482,8 +533,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                     }
                     more = 1;
                 }
-                umma_commit(&empty[slot]);
-                if (++slot == p.stages) { slot = 0; phase ^= 1; }
+                umma_commit(&empty[now]);
                 if (++kb == p.kblocks) kb = 0;
                 quantised += p.n * 128 + 1024;
             }
@@ -496,23 +546,10 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
         __syncwarp();
     } else {
         if (MX4 && fused) {
-            // Four lanes share a block of 32 values; the padding rows stay as they are (their columns are not stored), the columns past the
-            // last one become zero codes with a zero scale byte.
-            const uint32_t groups = (k1 - k0) * 32, tid = threadIdx.x - 64;            // groups of eight columns of this CTA's K
-            for (uint32_t i = tid; i < p.tokens * groups; i += 128) {
-                const uint32_t t = i / groups, c = i % groups, col = k0 * 256 + c * 8;
-                float v[8] = {};
-                if (col < p.cols) load8_any(p, uint64_t(t) * p.x_ld + col, v);
-                uint32_t top = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const uint32_t s = mx4_scale(top), block = c / 32, in = c % 32;       // in: which eight of the block's 256 columns
-                uint8_t* const b = ring_p + p.resident + block * (p.n * 128 + 1024);
-                *reinterpret_cast<uint32_t*>(b + t * 128 + (((in >> 2) ^ (t & 7)) << 4) + (in & 3) * 4) = mx4_codes8(v, s);
-                if ((in & 3) == 0) b[p.n * 128 + (in >> 4) * 512 + (t & 31) * 16 + (t >> 5) * 4 + ((in >> 2) & 3)] = uint8_t(s);
-            }
+            uint8_t* const to = ring_p + p.resident;
+            if (p.x_dtype == ZC_BF16) quantise_tokens<__nv_bfloat16>(p, k0, k1 - k0, to);
+            else if (p.x_dtype == ZC_F16) quantise_tokens<__half>(p, k0, k1 - k0, to);
+            else quantise_tokens<float>(p, k0, k1 - k0, to);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&tokens_ready);
         }
@@ -541,22 +578,21 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     if (p.splits > 1) {
         cluster_sync();
         if (warp >= 2 && !*abort_flag) {
-            const uint32_t row = threadIdx.x - 64;
-            for (uint32_t t = rank; t < p.tokens; t += p.splits) {
-                if (m0 + row >= p.M) break;
-                float v[MATS];
+            const uint32_t row = lane * 4;           // four rows a lane, a token a warp
+            for (uint32_t t = rank + (warp - 2) * p.splits; t < p.tokens; t += 4 * p.splits) {
+                float4 v[MATS];
 #pragma unroll
                 for (uint32_t i = 0; i < MATS; ++i) {
-                    float each[8];
+                    float4 each[8];
 #pragma unroll
                     for (uint32_t r = 0; r < 8; ++r)
                         if (r < p.splits) each[r] = load_peer(ring + ((i * p.tokens + t) * 128 + row) * 4, r);
                     v[i] = each[0];
 #pragma unroll
                     for (uint32_t r = 1; r < 8; ++r)
-                        if (r < p.splits) v[i] += each[r];
+                        if (r < p.splits) { v[i].x += each[r].x; v[i].y += each[r].y; v[i].z += each[r].z; v[i].w += each[r].w; }
                 }
-                few_store<MATS == 2>(p, uint64_t(t) * p.ldo + m0 + row, v[0], v[MATS - 1]);
+                few_store4<MATS == 2>(p, uint64_t(t) * p.ldo + m0 + row, m0 + row < p.M ? p.M - m0 - row : 0, v[0], v[MATS - 1]);
             }
         }
         __syncwarp();
@@ -681,7 +717,8 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     const int rc = configured.once(kernel, d.index, smem);
     if (rc != ZC_OK) return rc;
     void* const to[3] = {p.out[0], p.g ? p.g : p.out[1], p.u};
-    p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type));        // (the others are contiguous and aligned wherever they are given)
+    // A TMA store writes whole 16-byte pieces: rows start and end on one (the other outputs are contiguous and aligned wherever they are given).
+    p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && p.N * dtype_bytes(p.out_type) % 16 == 0;
     for (int i = 0; i < 3 && p.aligned; ++i)
         if (to[i] && !map_output(maps.o[i], to[i], p, GATED ? N / 4 : N / 2)) return no_maps();
     const uint32_t pairs = d.sms / 2;
@@ -711,7 +748,10 @@ template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block) {
 void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.n = (p.tokens + 15) / 16 * 16;
     const uint32_t total = p.kblocks * p.segs, mtiles = (p.M + TILE_M - 1) / TILE_M;
-    uint32_t splits = sms / mtiles;
+    // Two CTAs an SM: 8192 x 4096, one token 6.4 us, with one CTA an SM 7.5. Where the tiles alone fill three quarters of the SMs, more than sixteen
+    // tokens are not split: their sums cost more than the second CTA brings (16384 x 2048, 19 / 64 tokens 9.2 / 11.2 us, split in two 9.8 / 12.2; one
+    // token 7.2 and 6.5).
+    uint32_t splits = p.tokens > 16 && mtiles >= sms * 3 / 4 ? 1 : 2 * sms / mtiles;
     splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
     if (splits > total) splits = total;
     p.kown = (total + splits - 1) / splits;
@@ -738,6 +778,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
 
 template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, FewPlan& p, const Device& d, cudaStream_t s) {
     static Configured configured;
+    p.out_vec = rows16(p.out, p.ldo, dtype_bytes(p.out_type));
     auto kernel = few_kernel<MX4, A_MN, MATS>;
     const int rc = configured.once(kernel, d.index, FEW_SMEM_MAX);
     if (rc != ZC_OK) return rc;

@@ -14,6 +14,8 @@ for arguments, ``RuntimeError`` for the device.
 """
 import ctypes
 
+import torch
+
 from . import moe
 from .records import BF16, F16, F32
 
@@ -42,35 +44,32 @@ def load_library():
     return _lib
 
 
-def _torch():
-    import torch
-    return torch
+CODES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
 
 def _code(dtype, sixteen=False):
-    torch = _torch()
-    codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
-    if dtype not in codes or (sixteen and dtype == torch.float32):
+    if dtype not in CODES or (sixteen and dtype == torch.float32):
         raise ValueError(f"dtype must be {'bfloat16 or float16' if sixteen else 'bfloat16, float16 or float32'}, not {dtype}")
-    return codes[dtype]
+    return CODES[dtype]
 
 
 def _matrix(name, t, shape=None, dtype=None, contiguous=False):
     """Checks a matrix operand; -> its row stride in elements."""
-    torch = _torch()
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError(f"{name} must be a matrix")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     rows, cols = t.shape
+    if t.is_contiguous():
+        return cols
+    if contiguous:
+        raise ValueError(f"{name} must be contiguous")
     if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
         raise ValueError(f"{name} must have consecutive columns and rows that do not overlap")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
     return t.stride(0) if rows > 1 else cols
 
 
@@ -81,11 +80,14 @@ def _same_device(device, **others):
 
 
 def _call(device, name, *args):
-    """One library call on the device's current stream (its last argument)."""
-    torch = _torch()
+    """One library call on the device's current stream (its last argument), with that device current."""
     lib = load_library()
-    with torch.cuda.device(device):
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
     if rc != moe.ZC_OK:
         moe._raise(rc, lib.zc_last_error())
 
@@ -97,7 +99,7 @@ def _scale_bytes(rows, cols):
 def _out(out, rows, cols, dtype, device, name="out"):
     """The output matrix and its row stride."""
     if out is None:
-        out = _torch().empty((rows, cols), dtype=dtype, device=device)
+        out = torch.empty((rows, cols), dtype=dtype, device=device)
         return out, cols
     ld = _matrix(name, out, (rows, cols), dtype)
     _same_device(device, **{name: out})
@@ -109,7 +111,6 @@ class Mx4:
     tile layout of include/zc_ffn.h. Holds the tensors; copies nothing."""
 
     def __init__(self, codes, scales):
-        torch = _torch()
         if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
             raise ValueError("codes must be contiguous uint8 [rows, cols / 2], cols a multiple of 32")
         if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.device != codes.device or \
@@ -133,7 +134,6 @@ class Mx4:
 
     @staticmethod
     def empty(rows, cols, device):
-        torch = _torch()
         return Mx4(torch.empty((rows, cols // 2), dtype=torch.uint8, device=device), torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))
 
 
@@ -154,7 +154,6 @@ def mx4_quantize(x, out=None):
 
 def mx4_dequantize(q, dtype=None, out=None):
     """The values of an Mx4 (default bfloat16, which holds each of them exactly)."""
-    torch = _torch()
     dtype = out.dtype if dtype is None and out is not None else dtype or torch.bfloat16
     code = _code(dtype)
     out, ld = _out(out, q.rows, q.cols, dtype, q.device)
@@ -164,7 +163,6 @@ def mx4_dequantize(q, dtype=None, out=None):
 
 def mx4_from_rows(codes, scales):
     """A checkpoint's codes [rows, cols / 2] and row-major scales [rows, cols / 32] (both uint8) -> Mx4 (the codes are not copied)."""
-    torch = _torch()
     if scales.dim() != 2 or scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], codes.shape[-1] // 16):
         raise ValueError("scales must be contiguous uint8 [rows, cols / 32]")
     q = Mx4(codes, torch.empty(_scale_bytes(codes.shape[0], codes.shape[1] * 2), dtype=torch.uint8, device=codes.device))
@@ -174,7 +172,6 @@ def mx4_from_rows(codes, scales):
 
 
 def _mx4_product(entry, x, weights, out_dtype, out):
-    torch = _torch()
     w = weights[0]
     device, cols, rows = w.device, w.cols, w.rows
     for other in weights[1:]:
@@ -214,7 +211,6 @@ def mx4_gated(x, gate, up, out_dtype=None, out=None):
 def gated_forward(x, gate, up, save=False, out=None):
     """silu(x gate^T) * (x up^T): x [tokens, hidden], gate and up [ffn, hidden], one of bfloat16 and float16; -> h [tokens, ffn], and
     with ``save`` (h, g, u): the two products as gated_backward wants them."""
-    torch = _torch()
     code = _code(getattr(x, "dtype", None), sixteen=True)
     ld = _matrix("x", x)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
@@ -234,7 +230,6 @@ def gated_forward(x, gate, up, save=False, out=None):
 
 def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
     """The gradient of gated_forward -> (dx, dgate, dup) in the operands' dtype (None for what is not asked for)."""
-    torch = _torch()
     code = _code(getattr(x, "dtype", None), sixteen=True)
     x_ld = _matrix("x", x)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
@@ -257,7 +252,6 @@ def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
 
 def status(device=None):
     """Waits for the device's current stream and returns (then clears) the device's status word of these operators."""
-    torch = _torch()
     word = ctypes.c_uint32()
     lib = load_library()
     with torch.cuda.device(device):
