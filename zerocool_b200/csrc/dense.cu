@@ -58,7 +58,7 @@ struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
 struct TilePlan {
     uint32_t M, N;                      // rows and columns of an output (gated: N = ffn)
-    uint32_t kblocks, ksteps;           // blocks of 128 bytes of K; steps of 32 bytes in the last one
+    uint32_t kblocks, ksteps;           // stages of K; steps of 32 bytes in the last one
     uint32_t segs, outs;                // pairs (a[s], b[s]) whose products add up; outputs a[z] . b[0]
     uint32_t mtiles, ntiles, tiles;     // of 256 rows
     uint32_t idesc;
@@ -126,17 +126,21 @@ template <int NC> __device__ __forceinline__ void store_as(void* out, const CUte
     else if (p.out_type == ZC_F16) store_rows(static_cast<__half*>(out), map, p, row, col, patch, v);
     else if constexpr (NC >= 64) store_rows(static_cast<float*>(out), map, p, row, col, patch, v);      // (16-bit operands have 16-bit results)
 }
-__device__ __forceinline__ float silu(float v) { return __fdiv_rn(v, 1.0f + expf(-v)); }
+// The quotient by the fast reciprocal (2 ulp): with the rounded division the epilogue of a gated tile took 26,000 clocks, more than the products
+// of 3,300 k. A denominator beyond 2^126 gives 0, which is silu's limit there.
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
 
+// A stage is `depth` blocks of K, loaded and released together: a block is worth 256 to 512 clocks of products, and waiting for it, releasing it and
+// going round cost the issuing thread 300 beside its products' 40 each.
 template <bool MX4, int N> struct TileSmem {
-    static constexpr uint32_t b = N / 2 * 128, stage = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0);
-    static constexpr uint32_t stages = MX4 && N == 256 ? 5 : 6, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
+    static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = MX4 && N == 256 ? 1 : 2, stage = depth * block;
+    static constexpr uint32_t stages = depth == 1 ? 5 : MX4 || N == 256 ? 3 : 4, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
 };
 
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const TilePlan p) {
     typedef TileSmem<MX4, N> Smem;
-    constexpr uint32_t STAGES = Smem::stages, STAGE = Smem::stage, ACC = MX4 && N == 256 ? 1 : 2, SF_COLUMN = ACC * N;
+    constexpr uint32_t STAGES = Smem::stages, STAGE = Smem::stage, DEPTH = Smem::depth, ACC = MX4 && N == 256 ? 1 : 2, SF_COLUMN = ACC * N;
     constexpr uint32_t KB = MX4 ? 128 : 64;               // TMA elements of K a block (bytes of codes, 16-bit values)
     constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
     extern __shared__ uint8_t raw[];
@@ -176,26 +180,29 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : s];
                     const CUtensorMap* const mb = &maps.b[GATED ? rank : s];
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++it) {
-                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES;
                         if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
                         const uint32_t bar = map_to(smem_addr(&full[slot]), 0);             // the leader counts the bytes of both
                         if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
-                        if constexpr (A_MN) {
-                            for (uint32_t i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, ma, bar, row + i * 64, kb * 64);
-                        } else {
-                            tma_load_2d_pair(a, ma, bar, kb * KB, row);
-                        }
-                        if constexpr (B_MN) {
-                            for (uint32_t i = 0; i < N / 128; ++i) tma_load_2d_pair(b + i * 8192, mb, bar, col + i * 64, kb * 64);
-                        } else {
-                            tma_load_2d_pair(b, mb, bar, kb * KB, col);
-                        }
-                        if constexpr (MX4) {      // two scale tiles (256 k) of this CTA's rows of A and of all rows of B
-                            const uint32_t sf = b + Smem::b;
-                            const int at = (c.n0 / 128) * p.ktiles + kb * 2;
-                            tma_load_2d_pair(sf, &maps.sfa, bar, 0, (row / 128) * p.ktiles + kb * 2);
-                            tma_load_2d_pair(sf + 1024, &maps.sfb[0], bar, 0, at);
-                            if (N == 256) tma_load_2d_pair(sf + 2048, &maps.sfb[GATED ? 1 : 0], bar, 0, GATED ? at : at + p.ktiles);
+#pragma unroll
+                        for (uint32_t d = 0; d < DEPTH; ++d) {
+                            const uint32_t a = ring + slot * STAGE + d * Smem::block, b = a + A_BYTES, k = kb * DEPTH + d;      // k: block of K (one past the end is zeros)
+                            if constexpr (A_MN) {
+                                for (uint32_t i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, ma, bar, row + i * 64, k * 64);
+                            } else {
+                                tma_load_2d_pair(a, ma, bar, k * KB, row);
+                            }
+                            if constexpr (B_MN) {
+                                for (uint32_t i = 0; i < N / 128; ++i) tma_load_2d_pair(b + i * 8192, mb, bar, col + i * 64, k * 64);
+                            } else {
+                                tma_load_2d_pair(b, mb, bar, k * KB, col);
+                            }
+                            if constexpr (MX4) {      // two scale tiles (256 k) of this CTA's rows of A and of all rows of B
+                                const uint32_t sf = b + Smem::b;
+                                const int at = (c.n0 / 128) * p.ktiles + k * 2;
+                                tma_load_2d_pair(sf, &maps.sfa, bar, 0, (row / 128) * p.ktiles + k * 2);
+                                tma_load_2d_pair(sf + 1024, &maps.sfb[0], bar, 0, at);
+                                if (N == 256) tma_load_2d_pair(sf + 2048, &maps.sfb[GATED ? 1 : 0], bar, 0, GATED ? at : at + p.ktiles);
+                            }
                         }
                         if (++slot == STAGES) { slot = 0; ++round; }
                     }
@@ -221,35 +228,40 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 uint32_t more = 0;
                 for (uint32_t s = 0; ok && s < p.segs; ++s) {
                     for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-                        const uint32_t a = ring + slot * STAGE, b = a + A_BYTES, now = slot;
+                        const uint32_t stage = ring + slot * STAGE, now = slot;
                         if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         if (++slot == STAGES) { slot = 0; phase ^= 1; }
                         ready = mbar_test(&full[slot], phase);
-                        const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
-                        const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4;
-                        const uint32_t sf = tmem + SF_COLUMN + now * SF_COLUMNS;
-                        if constexpr (MX4) {
-                            // 128 k of scales: four columns for A's rows, four or eight for B's
-                            const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
+                        const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4 * DEPTH;
 #pragma unroll
-                            for (uint32_t j = 0; j < 2; ++j) {
-                                if (j * 2 >= steps) break;
-                                tmem_copy_scales_pair(sf + j * 4, ds + j * 32);
-#pragma unroll
-                                for (uint32_t i = 0; i < N / 128; ++i) tmem_copy_scales_pair(sf + 8 + j * 8 + i * 4, ds + 64 * (i + 1) + j * 32);
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            if (k >= steps) break;
+                        for (uint32_t d = 0; d < DEPTH; ++d) {
+                            if (d * 4 >= steps) break;
+                            const uint32_t a = stage + d * Smem::block, b = a + A_BYTES;
+                            const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
+                            const uint32_t sf = tmem + SF_COLUMN + now * SF_COLUMNS + d * (SF_COLUMNS / 2), sf_b = sf + 8, sf_step = N / 32;
                             if constexpr (MX4) {
-                                constexpr uint32_t odd = 2u << 29 | 2u << 4;      // the upper two of a column's four scales
-                                umma_mx4_pair(acc, da + k * 2, db + k * 2, k & 1 ? p.idesc | odd : p.idesc, sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8, more);
-                            } else {
-                                umma_f16_pair(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
+                                // 128 k of scales: four columns for A's rows, four or eight for B's
+                                const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
+#pragma unroll
+                                for (uint32_t j = 0; j < 2; ++j) {
+                                    if (d * 4 + j * 2 >= steps) break;
+                                    tmem_copy_scales_pair(sf + j * 4, ds + j * 32);
+#pragma unroll
+                                    for (uint32_t i = 0; i < N / 128; ++i) tmem_copy_scales_pair(sf_b + j * sf_step + i * 4, ds + 64 * (i + 1) + j * 32);
+                                }
                             }
-                            more = 1;
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                if (d * 4 + k >= steps) break;
+                                if constexpr (MX4) {
+                                    constexpr uint32_t odd = 2u << 29 | 2u << 4;      // the upper two of a column's four scales
+                                    umma_mx4_pair(acc, da + k * 2, db + k * 2, k & 1 ? p.idesc | odd : p.idesc, sf + (k >> 1) * 4, sf_b + (k >> 1) * sf_step, more);
+                                } else {
+                                    umma_f16_pair(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
+                                }
+                                more = 1;
+                            }
                         }
                         umma_commit_pair(&empty[now]);
                     }
@@ -738,9 +750,10 @@ bool narrow_tiles(TilePlan& p, const Device& d, uint32_t per_output) {
 }
 int too_many() { return fail(nullptr, ZC_EINVAL, "too many output tiles"); }
 
-template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block) {
+// K in blocks of `block` (`steps` steps of the tensor cores each); the steps of the last one.
+template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block, uint32_t steps = 4) {
     p.kblocks = (k + block - 1) / block;
-    const uint32_t left = k - (p.kblocks - 1) * block, step = block / 4;
+    const uint32_t left = k - (p.kblocks - 1) * block, step = block / steps;
     p.ksteps = (left + step - 1) / step;
 }
 
@@ -830,12 +843,13 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     if (x && (rc = launch_mx4_quantize(x, x_dtype, tokens, cols, x_ld, x_codes, x_scales, s)) != ZC_OK) return rc;
     TilePlan p{};
     p.M = tokens; p.N = rows; p.segs = 1; p.outs = 1;
-    set_k(p, cols, 256);
     p.ktiles = (cols + 127) / 128;
     p.out[0] = out; p.ldo = out_ld; p.out_type = out_dtype;
     const bool narrow = mats == 1 && narrow_tiles(p, d, 1);        // gated: 64 rows each of gate and up would share a scale tile
     const uint32_t n = narrow ? 128 : 256;
     if (!set_tiles(p, n / mats)) return too_many();
+    if (narrow) set_k(p, cols, 512, 8);
+    else set_k(p, cols, 256);
     p.idesc = idesc_mx4(256, n);
     if (!map_codes(maps.a[0], x_codes, tokens, cols, TILE_M) || !map_scales(maps.sfa, x_scales, tokens, cols)) return no_maps();
     for (int i = 0; i < mats; ++i)
@@ -903,7 +917,7 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
     }
     TilePlan p{};
     p.M = tokens; p.N = ffn; p.segs = 1; p.outs = 1;
-    set_k(p, hidden, 64);
+    set_k(p, hidden, 128, 8);
     p.out[0] = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
     const bool narrow = narrow_tiles(p, d, 2);
     const uint32_t n = narrow ? 128 : 256;
@@ -965,7 +979,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
         } else {
             TilePlan p{};
             p.M = tokens; p.N = hidden; p.segs = 2; p.outs = 1;
-            set_k(p, ffn, 64);
+            set_k(p, ffn, 128, 8);
             p.out[0] = dx; p.ldo = hidden; p.out_type = dtype;
             const bool narrow = narrow_tiles(p, d, 1);
             if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
@@ -980,7 +994,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
         TileMaps maps{};
         TilePlan p{};
         p.M = ffn; p.N = hidden; p.segs = 1; p.outs = 2;
-        set_k(p, tokens, 64);
+        set_k(p, tokens, 128, 8);
         p.out[0] = dgate; p.out[1] = dup; p.ldo = hidden; p.out_type = dtype;
         const bool narrow = narrow_tiles(p, d, 1);
         if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
