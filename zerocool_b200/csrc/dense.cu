@@ -54,6 +54,8 @@ constexpr uint32_t A_BYTES = TILE_M * 128;
 constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory columns of a stage's scales: A 2 x 4, B 2 x 8 at most
 constexpr uint32_t PATCH = 17, PATCH_BYTES = 4096;         // a warp's shared memory of the epilogue, and the floats of a row where it turns rows in it
 
+constexpr uint32_t SPLIT_STAGES = 3;                       // stages of K that a pair keeps where pairs share a tile
+
 struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
 struct TilePlan {
@@ -61,6 +63,7 @@ struct TilePlan {
     uint32_t kblocks, ksteps;           // stages of K; steps of 32 bytes in the last one
     uint32_t segs, outs;                // pairs (a[s], b[s]) whose products add up; outputs a[z] . b[0]
     uint32_t mtiles, ntiles, tiles;     // of 256 rows
+    uint32_t splits, kown;              // pairs that share a tile's K (then a cluster has one tile), stages of each
     uint32_t idesc;
     uint32_t ktiles;                    // MX4: scale tiles along K
     void* out[2];
@@ -79,11 +82,34 @@ __device__ __forceinline__ Tile tile_at(const TilePlan& p, uint32_t t, uint32_t 
     return {z, (band * 8 + j % rows) * 2 * TILE_M, j / rows * width};
 }
 
+// A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on, turned (at most) sixteen columns at a time through shared memory, so
+// that as many lanes store consecutive columns; rows past the last one and columns past it are left out.
+template <typename T, int NC> __device__ __forceinline__ void store_turned(T* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    constexpr int TURN = NC < 16 ? NC : 16;
+    float* const turned = reinterpret_cast<float*>(patch);
+    const uint32_t lane = threadIdx.x & 31;
+    if (row >= p.M) return;
+    const uint32_t rows = min(32u, p.M - row);
+#pragma unroll
+    for (int c = 0; c < NC; c += TURN) {
+#pragma unroll
+        for (int j = 0; j < TURN; ++j) turned[lane * PATCH + j] = v[c + j];
+        __syncwarp();
+        const uint32_t at = col + c + lane % TURN;
+        if (at < p.N)
+            for (uint32_t r = lane / TURN; r < rows; r += 32 / TURN) out[uint64_t(row + r) * p.ldo + at] = from_f32<T>(turned[r * PATCH + lane % TURN]);
+        __syncwarp();
+    }
+}
+template <int NC> __device__ __forceinline__ void store_turned_as(void* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    if (p.out_type == ZC_BF16) store_turned(static_cast<__nv_bfloat16*>(out), p, row, col, patch, v);
+    else if (p.out_type == ZC_F16) store_turned(static_cast<__half*>(out), p, row, col, patch, v);
+    else store_turned(static_cast<float*>(out), p, row, col, patch, v);
+}
 // A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on; rows past `rows` and columns past `cols` are left out. Rows that
 // are 16-byte aligned leave by TMA: 128 (or 64) bytes of each through shared memory, swizzled so that neither side meets a bank twice.
 // Stored by the lanes, 16 bytes of a row each, they took 6,200 clocks a tile, and the waits of the copying and the issuing
-// thread queued behind them. Rows that are not aligned are turned sixteen columns at a time through the same memory, so that
-// sixteen lanes store consecutive columns (257 x 10007: 45 -> 23 us against values stored by the rows' own lanes).
+// thread queued behind them. Rows that are not aligned are turned (257 x 10007: 45 -> 23 us against values stored by the rows' own lanes).
 template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
     const uint32_t lane = threadIdx.x & 31;
     if (row >= p.M) return;
@@ -108,18 +134,7 @@ template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out,
         }
         return;
     }
-    float* const turned = reinterpret_cast<float*>(patch);
-    const uint32_t rows = min(32u, p.M - row);
-#pragma unroll
-    for (int c = 0; c < NC; c += 16) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) turned[lane * PATCH + j] = v[c + j];
-        __syncwarp();
-        const uint32_t at = col + c + (lane & 15);
-        if (at < p.N)
-            for (uint32_t r = lane >> 4; r < rows; r += 2) out[uint64_t(row + r) * p.ldo + at] = from_f32<T>(turned[r * PATCH + (lane & 15)]);
-        __syncwarp();
-    }
+    store_turned(out, p, row, col, patch, v);
 }
 template <int NC> __device__ __forceinline__ void store_as(void* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
     if (p.out_type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
@@ -130,11 +145,11 @@ template <int NC> __device__ __forceinline__ void store_as(void* out, const CUte
 // of 3,300 k. A denominator beyond 2^126 gives 0, which is silu's limit there.
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
 
-// A stage is `depth` blocks of K, loaded and released together: a block is worth 256 to 512 clocks of products, and waiting for it, releasing it and
-// going round cost the issuing thread 300 beside its products' 40 each.
+// A stage is `depth` blocks of K, loaded and released together: with 128 columns a block is worth 256 clocks of products, and waiting for it,
+// releasing it and going round cost the issuing thread 300 beside its products' 40 each.
 template <bool MX4, int N> struct TileSmem {
-    static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = MX4 && N == 256 ? 1 : 2, stage = depth * block;
-    static constexpr uint32_t stages = depth == 1 ? 5 : MX4 || N == 256 ? 3 : 4, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
+    static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = N == 256 ? 1 : 2, stage = depth * block;
+    static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
 };
 
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
@@ -147,7 +162,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t rank = blockIdx.x & 1, part = (blockIdx.x >> 1) % p.splits, lead = part * 2;       // lead: the leader's rank in the cluster
+    const uint32_t pair = (blockIdx.x >> 1) / p.splits, pairs = (gridDim.x >> 1) / p.splits;
+    const uint32_t k0 = part * p.kown, k1 = min(k0 + p.kown, p.segs * p.kblocks);                     // of the stages of all segments
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
     if (threadIdx.x == 0) {
@@ -176,36 +193,36 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 const Tile c = tile_at(p, t, WIDTH);
                 const int row = c.m0 + rank * TILE_M;                                       // of A
                 const int col = GATED ? c.n0 : c.n0 + rank * (N / 2);                       // row of B (gated: the leader has gate's, the other up's)
-                for (uint32_t s = 0; ok && s < p.segs; ++s) {
-                    const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : s];
-                    const CUtensorMap* const mb = &maps.b[GATED ? rank : s];
-                    for (uint32_t kb = 0; kb < p.kblocks; ++kb, ++it) {
-                        if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
-                        const uint32_t bar = map_to(smem_addr(&full[slot]), 0);             // the leader counts the bytes of both
-                        if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
+                uint32_t seg = k0 / p.kblocks, kb = k0 % p.kblocks;
+                for (uint32_t left = k1 - k0; left; --left, ++it) {
+                    const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : seg];
+                    const CUtensorMap* const mb = &maps.b[GATED ? rank : seg];
+                    if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
+                    const uint32_t bar = map_to(smem_addr(&full[slot]), lead);          // the leader counts the bytes of both
+                    if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
 #pragma unroll
-                        for (uint32_t d = 0; d < DEPTH; ++d) {
-                            const uint32_t a = ring + slot * STAGE + d * Smem::block, b = a + A_BYTES, k = kb * DEPTH + d;      // k: block of K (one past the end is zeros)
-                            if constexpr (A_MN) {
-                                for (uint32_t i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, ma, bar, row + i * 64, k * 64);
-                            } else {
-                                tma_load_2d_pair(a, ma, bar, k * KB, row);
-                            }
-                            if constexpr (B_MN) {
-                                for (uint32_t i = 0; i < N / 128; ++i) tma_load_2d_pair(b + i * 8192, mb, bar, col + i * 64, k * 64);
-                            } else {
-                                tma_load_2d_pair(b, mb, bar, k * KB, col);
-                            }
-                            if constexpr (MX4) {      // two scale tiles (256 k) of this CTA's rows of A and of all rows of B
-                                const uint32_t sf = b + Smem::b;
-                                const int at = (c.n0 / 128) * p.ktiles + k * 2;
-                                tma_load_2d_pair(sf, &maps.sfa, bar, 0, (row / 128) * p.ktiles + k * 2);
-                                tma_load_2d_pair(sf + 1024, &maps.sfb[0], bar, 0, at);
-                                if (N == 256) tma_load_2d_pair(sf + 2048, &maps.sfb[GATED ? 1 : 0], bar, 0, GATED ? at : at + p.ktiles);
-                            }
+                    for (uint32_t d = 0; d < DEPTH; ++d) {
+                        const uint32_t a = ring + slot * STAGE + d * Smem::block, b = a + A_BYTES, k = kb * DEPTH + d;      // k: block of K (one past the end is zeros)
+                        if constexpr (A_MN) {
+                            for (uint32_t i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, ma, bar, row + i * 64, k * 64);
+                        } else {
+                            tma_load_2d_pair(a, ma, bar, k * KB, row);
                         }
-                        if (++slot == STAGES) { slot = 0; ++round; }
+                        if constexpr (B_MN) {
+                            for (uint32_t i = 0; i < N / 128; ++i) tma_load_2d_pair(b + i * 8192, mb, bar, col + i * 64, k * 64);
+                        } else {
+                            tma_load_2d_pair(b, mb, bar, k * KB, col);
+                        }
+                        if constexpr (MX4) {      // two scale tiles (256 k) of this CTA's rows of A and of all rows of B
+                            const uint32_t sf = b + Smem::b;
+                            const int at = (c.n0 / 128) * p.ktiles + k * 2;
+                            tma_load_2d_pair(sf, &maps.sfa, bar, 0, (row / 128) * p.ktiles + k * 2);
+                            tma_load_2d_pair(sf + 1024, &maps.sfb[0], bar, 0, at);
+                            if (N == 256) tma_load_2d_pair(sf + 2048, &maps.sfb[GATED ? 1 : 0], bar, 0, GATED ? at : at + p.ktiles);
+                        }
                     }
+                    if (++slot == STAGES) { slot = 0; ++round; }
+                    if (++kb == p.kblocks) { kb = 0; ++seg; }
                 }
             }
             if (!ok) {        // the last copies land before the CTA may end: the leader's barriers count those of both
@@ -225,51 +242,50 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 const uint32_t buf = n % ACC, acc = tmem + buf * N;
                 if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t more = 0;
-                for (uint32_t s = 0; ok && s < p.segs; ++s) {
-                    for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-                        const uint32_t stage = ring + slot * STAGE, now = slot;
-                        if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
-                        ready = mbar_test(&full[slot], phase);
-                        const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4 * DEPTH;
+                uint32_t more = 0, kb = k0 % p.kblocks;
+                for (uint32_t left = k1 - k0; left; --left) {
+                    const uint32_t stage = ring + slot * STAGE, now = slot;
+                    if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (++slot == STAGES) { slot = 0; phase ^= 1; }
+                    ready = mbar_test(&full[slot], phase);
+                    const uint32_t steps = kb + 1 == p.kblocks ? p.ksteps : 4 * DEPTH;
 #pragma unroll
-                        for (uint32_t d = 0; d < DEPTH; ++d) {
-                            if (d * 4 >= steps) break;
-                            const uint32_t a = stage + d * Smem::block, b = a + A_BYTES;
-                            const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
-                            const uint32_t sf = tmem + SF_COLUMN + now * SF_COLUMNS + d * (SF_COLUMNS / 2), sf_b = sf + 8, sf_step = N / 32;
-                            if constexpr (MX4) {
-                                // 128 k of scales: four columns for A's rows, four or eight for B's
-                                const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
+                    for (uint32_t d = 0; d < DEPTH; ++d) {
+                        if (d * 4 >= steps) break;
+                        const uint32_t a = stage + d * Smem::block, b = a + A_BYTES;
+                        const uint64_t da = desc_at(A_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, a), db = desc_at(B_MN ? DESC_MN_MAJOR : DESC_K_MAJOR, b);
+                        const uint32_t sf = tmem + SF_COLUMN + now * SF_COLUMNS + d * (SF_COLUMNS / 2), sf_b = sf + 8, sf_step = N / 32;
+                        if constexpr (MX4) {
+                            // 128 k of scales: four columns for A's rows, four or eight for B's
+                            const uint64_t ds = desc_at(DESC_SCALES, b + Smem::b);
 #pragma unroll
-                                for (uint32_t j = 0; j < 2; ++j) {
-                                    if (d * 4 + j * 2 >= steps) break;
-                                    tmem_copy_scales_pair(sf + j * 4, ds + j * 32);
+                            for (uint32_t j = 0; j < 2; ++j) {
+                                if (d * 4 + j * 2 >= steps) break;
+                                tmem_copy_scales_pair(sf + j * 4, ds + j * 32);
 #pragma unroll
-                                    for (uint32_t i = 0; i < N / 128; ++i) tmem_copy_scales_pair(sf_b + j * sf_step + i * 4, ds + 64 * (i + 1) + j * 32);
-                                }
-                            }
-#pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k) {
-                                if (d * 4 + k >= steps) break;
-                                if constexpr (MX4) {
-                                    constexpr uint32_t odd = 2u << 29 | 2u << 4;      // the upper two of a column's four scales
-                                    umma_mx4_pair(acc, da + k * 2, db + k * 2, k & 1 ? p.idesc | odd : p.idesc, sf + (k >> 1) * 4, sf_b + (k >> 1) * sf_step, more);
-                                } else {
-                                    umma_f16_pair(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
-                                }
-                                more = 1;
+                                for (uint32_t i = 0; i < N / 128; ++i) tmem_copy_scales_pair(sf_b + j * sf_step + i * 4, ds + 64 * (i + 1) + j * 32);
                             }
                         }
-                        umma_commit_pair(&empty[now]);
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            if (d * 4 + k >= steps) break;
+                            if constexpr (MX4) {
+                                constexpr uint32_t odd = 2u << 29 | 2u << 4;      // the upper two of a column's four scales
+                                umma_mx4_pair(acc, da + k * 2, db + k * 2, k & 1 ? p.idesc | odd : p.idesc, sf + (k >> 1) * 4, sf_b + (k >> 1) * sf_step, more);
+                            } else {
+                                umma_f16_pair(acc, da + k * (A_MN ? 128 : 2), db + k * (B_MN ? 128 : 2), p.idesc, more);
+                            }
+                            more = 1;
+                        }
                     }
+                    if (++kb == p.kblocks) kb = 0;
+                    umma_commit_pair(&empty[now], lead);
                 }
-                if (ok) umma_commit_pair(&acc_full[buf]);
+                if (ok) umma_commit_pair(&acc_full[buf], lead);
             }
             if (abort_s) {       // products in flight read shared memory and write tensor memory: they end first
-                umma_commit_pair(&drain);
+                umma_commit_pair(&drain, lead);
                 for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
             }
         }
@@ -293,8 +309,18 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(map_to(smem_addr(&acc_empty[buf]), 0));
+            if (lane == 0) mbar_arrive_at(map_to(smem_addr(&acc_empty[buf]), lead));
             const uint32_t row = c.m0 + rank * TILE_M + quarter * 32, col = c.n0 + half * COLS;
+            if (N == 128 && p.splits > 1) {
+                // The sums of this part of K, [column][row]; every stage of the ring has been read.
+                float* const mine = reinterpret_cast<float*>(raw + (ring - smem_addr(raw))) + half * COLS * TILE_M + quarter * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) {
+                    mine[i * TILE_M] = v[i];
+                    if constexpr (GATED) mine[(N / 2 + i) * TILE_M] = w[i];
+                }
+                continue;
+            }
             if constexpr (GATED) {
                 if (p.g) {
                     store_as(p.g, &maps.o[1], p, row, col, patch, v);
@@ -307,6 +333,41 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
         if (lane == 0) tma_store_done();
         __syncwarp();
+    }
+    if constexpr (N == 128) {
+        if (p.splits > 1) {
+            // Every pair adds a part of the tile's columns over the pairs, in their order, eight columns a warp at a time.
+            cluster_sync();
+            if (warp >= 2 && __all_sync(0xffffffffu, !*abort_flag)) {
+                const uint32_t quarter = warp & 3, share = WIDTH / p.splits;
+                uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * PATCH_BYTES;
+                const Tile c = tile_at(p, pair, WIDTH);
+                const uint32_t row = c.m0 + rank * TILE_M + quarter * 32;
+                for (uint32_t j = part * share + ((warp - 2) >> 2) * 8; j < (part + 1) * share; j += 16) {
+                    float v[8], w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = w[i] = 0.0f;
+                    for (uint32_t r = 0; r < p.splits; ++r) {
+                        const uint32_t from = map_to(ring + (j * TILE_M + quarter * 32 + lane) * 4, r * 2 + rank);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[i] += load_cluster(from + i * TILE_M * 4);
+                            if constexpr (GATED) w[i] += load_cluster(from + (N / 2 + i) * TILE_M * 4);
+                        }
+                    }
+                    if constexpr (GATED) {
+                        if (p.g) {
+                            store_turned_as(p.g, p, row, c.n0 + j, patch, v);
+                            store_turned_as(p.u, p, row, c.n0 + j, patch, w);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = silu(v[i]) * w[i];
+                    }
+                    store_turned_as(c.z ? p.out[1] : p.out[0], p, row, c.n0 + j, patch, v);
+                }
+            }
+            __syncwarp();
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync();
@@ -710,14 +771,25 @@ bool map_output(CUtensorMap& m, void* out, const TilePlan& p, uint32_t columns) 
                   columns < most ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The opt-in to large shared memory of one kernel, once per device.
+// The opt-in to large shared memory of one kernel, and the clusters of 4 and 8 CTAs of it that the device holds at a time, once per device.
 struct Configured {
     std::atomic<bool> done[MAX_DEVICES] = {};
-    template <typename Kernel> int once(Kernel kernel, int device, size_t smem) {
-        if (done[device].load(std::memory_order_relaxed)) return ZC_OK;
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-        if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e)); }
-        done[device].store(true, std::memory_order_relaxed);
+    std::atomic<uint32_t> clusters[MAX_DEVICES][2] = {};
+    template <typename Kernel> int once(Kernel kernel, int device, size_t smem, uint32_t threads, bool count) {
+        if (done[device].load(std::memory_order_acquire)) return ZC_OK;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        for (int i = 0; e == cudaSuccess && count && i < 2; ++i) {
+            cudaLaunchConfig_t cfg{};
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 4u << i; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+            cfg.gridDim = dim3(4u << i); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.attrs = &attr; cfg.numAttrs = 1;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+            clusters[device][i].store(uint32_t(n), std::memory_order_relaxed);
+        }
+        if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("dense product set-up: ") + cudaGetErrorString(e)); }
+        done[device].store(true, std::memory_order_release);
         return ZC_OK;
     }
 };
@@ -726,15 +798,20 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     static Configured configured;
     auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED, N>;
     constexpr uint32_t smem = TileSmem<MX4, N>::bytes;
-    const int rc = configured.once(kernel, d.index, smem);
+    const int rc = configured.once(kernel, d.index, smem, THREADS, N == 128);
     if (rc != ZC_OK) return rc;
     void* const to[3] = {p.out[0], p.g ? p.g : p.out[1], p.u};
     // A TMA store writes whole 16-byte pieces: rows start and end on one (the other outputs are contiguous and aligned wherever they are given).
     p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && p.N * dtype_bytes(p.out_type) % 16 == 0;
     for (int i = 0; i < 3 && p.aligned; ++i)
         if (to[i] && !map_output(maps.o[i], to[i], p, GATED ? N / 4 : N / 2)) return no_maps();
-    const uint32_t pairs = d.sms / 2;
-    return launched(launch_after(kernel, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), THREADS, smem, 2, s, maps, p), "dense product");
+    const uint32_t pairs = d.sms / 2, total = p.segs * p.kblocks;
+    // K is shared by two or four pairs where all of the tiles still run at once: dx of 300 x 2048 x 8192 58 -> 39 us; MX4 256 x 2048 x 8192 10.8 us
+    // with two pairs a tile, 17.5 with four, whose sixteen clusters do not all fit.
+    p.splits = 1;
+    for (int i = 0; N == 128 && i < 2 && p.tiles <= configured.clusters[d.index][i] && total >= (2u << i) * SPLIT_STAGES; ++i) p.splits = 2u << i;
+    p.kown = (total + p.splits - 1) / p.splits;
+    return launched(launch_after(kernel, dim3(2 * p.splits * (p.splits > 1 || p.tiles < pairs ? p.tiles : pairs)), THREADS, smem, 2 * p.splits, s, maps, p), "dense product");
 }
 
 // Tiles of `width` output columns; the number of them, or 0 where there are too many.
@@ -756,6 +833,7 @@ template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block, uint32_
     const uint32_t left = k - (p.kblocks - 1) * block, step = block / steps;
     p.ksteps = (left + step - 1) / step;
 }
+void set_tile_k(TilePlan& p, uint32_t k, uint32_t block, bool narrow) { narrow ? set_k(p, k, 2 * block, 8) : set_k(p, k, block); }
 
 // Cuts a call of few tokens (at most FEW_TOKENS). kblocks, ksteps, segs, M, tokens, cols are set; plain: x is to be quantised.
 void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
@@ -793,7 +871,7 @@ template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, Fe
     static Configured configured;
     p.out_vec = rows16(p.out, p.ldo, dtype_bytes(p.out_type));
     auto kernel = few_kernel<MX4, A_MN, MATS>;
-    const int rc = configured.once(kernel, d.index, FEW_SMEM_MAX);
+    const int rc = configured.once(kernel, d.index, FEW_SMEM_MAX, FEW_THREADS, false);
     if (rc != ZC_OK) return rc;
     return launched(launch_after(kernel, dim3((p.M + TILE_M - 1) / TILE_M * p.splits), FEW_THREADS, p.smem, p.splits, s, maps, p), "dense product of few tokens");
 }
@@ -848,8 +926,7 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     const bool narrow = mats == 1 && narrow_tiles(p, d, 1);        // gated: 64 rows each of gate and up would share a scale tile
     const uint32_t n = narrow ? 128 : 256;
     if (!set_tiles(p, n / mats)) return too_many();
-    if (narrow) set_k(p, cols, 512, 8);
-    else set_k(p, cols, 256);
+    set_tile_k(p, cols, 256, narrow);
     p.idesc = idesc_mx4(256, n);
     if (!map_codes(maps.a[0], x_codes, tokens, cols, TILE_M) || !map_scales(maps.sfa, x_scales, tokens, cols)) return no_maps();
     for (int i = 0; i < mats; ++i)
@@ -917,9 +994,9 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
     }
     TilePlan p{};
     p.M = tokens; p.N = ffn; p.segs = 1; p.outs = 1;
-    set_k(p, hidden, 128, 8);
     p.out[0] = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
     const bool narrow = narrow_tiles(p, d, 2);
+    set_tile_k(p, hidden, 64, narrow);
     const uint32_t n = narrow ? 128 : 256;
     if (!set_tiles(p, n / 2)) return too_many();
     p.idesc = idesc_f16(dtype, false, false, 256, n);
@@ -979,9 +1056,9 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
         } else {
             TilePlan p{};
             p.M = tokens; p.N = hidden; p.segs = 2; p.outs = 1;
-            set_k(p, ffn, 128, 8);
             p.out[0] = dx; p.ldo = hidden; p.out_type = dtype;
             const bool narrow = narrow_tiles(p, d, 1);
+            set_tile_k(p, ffn, 64, narrow);
             if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
             p.idesc = idesc_f16(dtype, false, true, 256, narrow ? 128 : 256);
             if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, TILE_M) || !map_rows(maps.a[1], du, tokens, ffn, ffn, TILE_M) ||
@@ -994,9 +1071,9 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
         TileMaps maps{};
         TilePlan p{};
         p.M = ffn; p.N = hidden; p.segs = 1; p.outs = 2;
-        set_k(p, tokens, 128, 8);
         p.out[0] = dgate; p.out[1] = dup; p.ldo = hidden; p.out_type = dtype;
         const bool narrow = narrow_tiles(p, d, 1);
+        set_tile_k(p, tokens, 64, narrow);
         if (!set_tiles(p, narrow ? 128 : 256)) return too_many();
         p.idesc = idesc_f16(dtype, true, true, 256, narrow ? 128 : 256);
         if (!map_rows(maps.a[0], dg, tokens, ffn, ffn, ACROSS) || !map_rows(maps.a[1], du, tokens, ffn, ffn, ACROSS) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, ACROSS)) return no_maps();

@@ -149,8 +149,13 @@ __device__ __forceinline__ void umma_mx4_pair(uint32_t tmem_d, uint64_t adesc, u
 __device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {      // arrives at this barrier of both CTAs
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"(uint16_t(3)) : "memory");
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t lead) {      // arrives at this barrier of both CTAs, ranks lead and lead + 1
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"(uint16_t(3u << lead)) : "memory");
+}
+__device__ __forceinline__ float load_cluster(uint32_t addr) {      // an address of map_to
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {      // a group of its own
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
