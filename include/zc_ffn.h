@@ -62,9 +62,10 @@ int zc_mx4_gated(const void* x, int x_dtype, uint64_t x_ld, void* x_codes, void*
 
 /* The gated block in 16 bits. x [tokens, hidden] (row stride x_ld), gate and up [ffn, hidden], all of one dtype (BF16 or F16), hidden and
  * ffn multiples of 8. h [tokens, ffn] = silu(x . gate^T) * (x . up^T), rounded once from FP32. g and u (both or neither): the two products
- * themselves, [tokens, ffn] in dtype, for zc_gated_backward. */
+ * themselves, [tokens, ffn], for zc_gated_backward: in FP32 (saved_dtype ZC_F32), or rounded to dtype (saved_dtype = dtype), which halves what
+ * is kept between the two calls and adds two roundings of dtype to the gradients' error. */
 int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void* up, int dtype, uint32_t tokens, uint32_t hidden, uint32_t ffn,
-                     void* h, void* g, void* u, void* stream);
+                     void* h, void* g, void* u, int saved_dtype, void* stream);
 
 /* Its gradient: dh [tokens, ffn] (row stride dh_ld) and what zc_gated_forward was given and gave.
  *   s = sigmoid(g);  dg = dh u s (1 + g (1 - s));  du = dh g s
@@ -72,7 +73,7 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
  * dg and du [tokens, ffn] are written too (the operands of the products, rounded to dtype); dx or both of dgate and dup may be NULL
  * where they are not wanted. dx, dgate and dup are rounded once from FP32 sums. */
 int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_ld, const void* gate, const void* up, const void* g, const void* u,
-                      int dtype, uint32_t tokens, uint32_t hidden, uint32_t ffn, void* dg, void* du, void* dx, void* dgate, void* dup, void* stream);
+                      int saved_dtype, int dtype, uint32_t tokens, uint32_t hidden, uint32_t ffn, void* dg, void* du, void* dx, void* dgate, void* dup, void* stream);
 
 /* Waits for `stream` and returns the current device's status word of these operators (then clears it). */
 int zc_ffn_status(void* stream, uint32_t* status);

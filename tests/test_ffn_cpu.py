@@ -48,12 +48,12 @@ def gated4(x=None, xc=at(0), xs=at(1), tokens=4, cols=64, gc=at(2), gs=at(3), uc
     return ffn.load_library().zc_mx4_gated(x, F32, cols, xc, xs, tokens, cols, gc, gs, uc, us, ffn_, out, out_dtype, out_ld, None)
 
 
-def forward(x=at(0), x_ld=16, gate=at(1), up=at(2), dtype=BF16, tokens=4, hidden=16, ffn_=8, h=at(3), g=at(4), u=at(5)):
-    return ffn.load_library().zc_gated_forward(x, x_ld, gate, up, dtype, tokens, hidden, ffn_, h, g, u, None)
+def forward(x=at(0), x_ld=16, gate=at(1), up=at(2), dtype=BF16, tokens=4, hidden=16, ffn_=8, h=at(3), g=at(4), u=at(5), saved=F32):
+    return ffn.load_library().zc_gated_forward(x, x_ld, gate, up, dtype, tokens, hidden, ffn_, h, g, u, saved, None)
 
 
-def backward(dh=at(0), dh_ld=8, x=at(1), x_ld=16, gate=at(2), up=at(3), g=at(4), u=at(5), dtype=BF16, tokens=4, hidden=16, ffn_=8, dg=at(6), du=at(7), dx=at(8), dgate=at(9), dup=at(10)):
-    return ffn.load_library().zc_gated_backward(dh, dh_ld, x, x_ld, gate, up, g, u, dtype, tokens, hidden, ffn_, dg, du, dx, dgate, dup, None)
+def backward(dh=at(0), dh_ld=8, x=at(1), x_ld=16, gate=at(2), up=at(3), g=at(4), u=at(5), dtype=BF16, tokens=4, hidden=16, ffn_=8, dg=at(6), du=at(7), dx=at(8), dgate=at(9), dup=at(10), saved=F32):
+    return ffn.load_library().zc_gated_backward(dh, dh_ld, x, x_ld, gate, up, g, u, saved, dtype, tokens, hidden, ffn_, dg, du, dx, dgate, dup, None)
 
 
 @pytest.mark.parametrize("call,why", [
@@ -71,6 +71,8 @@ def backward(dh=at(0), dh_ld=8, x=at(1), x_ld=16, gate=at(2), up=at(3), g=at(4),
     (lambda: forward(dtype=F32), b"dtype"), (lambda: forward(hidden=20, x_ld=24), b"multiples of 8"), (lambda: forward(ffn_=12), b"multiples of 8"), (lambda: forward(x_ld=20), b"multiple of 16 bytes"),
     (lambda: forward(x_ld=8), b"row stride"), (lambda: forward(u=None), b"go together"), (lambda: forward(g=None), b"go together"), (lambda: forward(x=at(0) + 2), b"16-byte aligned"),
     (lambda: forward(gate=None), b"missing buffer"), (lambda: forward(h=at(1)), b"overlapping"), (lambda: forward(g=at(3) + 16), b"overlapping"),
+    (lambda: forward(saved=F16), b"g and u must be"), (lambda: forward(saved=7), b"g and u must be"), (lambda: forward(u=at(4) + 64), b"overlapping"), (lambda: forward(g=at(4) + 4), b"16-byte aligned"),
+    (lambda: backward(saved=F16), b"g and u must be"), (lambda: backward(dx=at(4) + 96), b"overlapping"),
     (lambda: backward(dtype=F32), b"dtype"), (lambda: backward(dh_ld=12), b"multiple of 16 bytes"), (lambda: backward(dup=None), b"go together"), (lambda: backward(dg=None), b"missing buffer"),
     (lambda: backward(du=at(6)), b"overlapping"), (lambda: backward(dx=at(1)), b"overlapping"), (lambda: backward(dgate=at(2)), b"overlapping"), (lambda: backward(tokens=1 << 31), b"shape"),
 ])

@@ -214,7 +214,10 @@ def test_gated_forward(ffn, tokens, hidden, width, dtype):
     close(g, gw, gs)
     close(u, uw, us)
     close(h, ref.silu(gw) * uw, 1.1 * gs * uw.abs() + ref.silu(gw).abs() * us + 1.1 * gs * us + 2.0 ** -20 * (ref.silu(gw) * uw).abs())
+    assert g.dtype == u.dtype == torch.float32
     assert torch.equal(h, ffn.gated_forward(view_of(x, 8), gate, up))
+    small = ffn.gated_forward(x, gate, up, save=True, save_dtype=dtype)
+    assert torch.equal(small[0], h) and torch.equal(small[1], g.to(dtype)) and torch.equal(small[2], u.to(dtype))
 
 
 def gradient_slack(dtype, dh, x, gate, up, g, u):
@@ -235,11 +238,12 @@ def gradient_slack(dtype, dh, x, gate, up, g, u):
 def test_gated_backward(ffn, tokens, hidden, width, dtype):
     x, gate, up = randn((tokens, hidden), 1, dtype=dtype), randn((width, hidden), 2, 0.2, dtype), randn((width, hidden), 3, 0.2, dtype)
     dh = randn((tokens, width), 4, 0.5, dtype)
-    _, g, u = ffn.gated_forward(x, gate, up, save=True)
-    d = [t.double() for t in (dh, x, gate, up, g, u)]
-    got = ffn.gated_backward(dh, x, gate, up, g, u)
-    for name, a, b, slack in zip(("dx", "dgate", "dup"), got, ref.gated_gradient(*d)[2:], gradient_slack(dtype, *d)):
-        close(a, b, slack, name)
+    for saved in (dtype, torch.float32):
+        _, g, u = ffn.gated_forward(x, gate, up, save=True, save_dtype=saved)
+        d = [t.double() for t in (dh, x, gate, up, g, u)]
+        got = ffn.gated_backward(dh, x, gate, up, g, u)
+        for name, a, b, slack in zip(("dx", "dgate", "dup"), got, ref.gated_gradient(*d)[2:], gradient_slack(dtype, *d)):
+            close(a, b, slack, name)
     again = ffn.gated_backward(view_of(dh, 8), view_of(x, 8), gate, up, g, u)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
     only_x = ffn.gated_backward(dh, x, gate, up, g, u, weight_grads=False)
@@ -339,6 +343,7 @@ def test_python_refusals(ffn):
                       (lambda: ffn.Mx4(w.codes[:, :8], w.scales), "codes"), (lambda: ffn.Mx4(w.codes, w.scales[:256]), "scales"),
                       (lambda: ffn.mx4_from_rows(w.codes, torch.zeros(8, 3, dtype=torch.uint8, device="cuda")), "scales"),
                       (lambda: ffn.gated_forward(x.bfloat16(), x.half(), x.half()), "gate must be"), (lambda: ffn.gated_forward(x.half(), x.half()[:, :32], x.half()), "gate must be"),
+                      (lambda: ffn.gated_forward(x.half(), x.half(), x.half(), save=True, save_dtype=torch.bfloat16), "save_dtype"),
                       (lambda: ffn.gated_forward(x.half()[:, :20], x.half()[:, :20].contiguous(), x.half()[:, :20].contiguous()), "multiples of 8")):
         with pytest.raises(ValueError, match=why):
             call()

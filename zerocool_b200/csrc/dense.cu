@@ -69,7 +69,7 @@ struct TilePlan {
     void* out[2];
     uint64_t ldo;
     void *g, *u;                        // gated: where the two products go as well, or null
-    int out_type;
+    int out_type, saved_type;           // of the outputs; of g and u
     bool aligned;                       // the output's rows start and end on 16 bytes: o[] are views of out[0], and of out[1], or of g and u
 };
 
@@ -101,9 +101,9 @@ template <typename T, int NC> __device__ __forceinline__ void store_turned(T* ou
         __syncwarp();
     }
 }
-template <int NC> __device__ __forceinline__ void store_turned_as(void* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
-    if (p.out_type == ZC_BF16) store_turned(static_cast<__nv_bfloat16*>(out), p, row, col, patch, v);
-    else if (p.out_type == ZC_F16) store_turned(static_cast<__half*>(out), p, row, col, patch, v);
+template <int NC> __device__ __forceinline__ void store_turned_as(void* out, int type, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    if (type == ZC_BF16) store_turned(static_cast<__nv_bfloat16*>(out), p, row, col, patch, v);
+    else if (type == ZC_F16) store_turned(static_cast<__half*>(out), p, row, col, patch, v);
     else store_turned(static_cast<float*>(out), p, row, col, patch, v);
 }
 // A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on; rows past `rows` and columns past `cols` are left out. Rows that
@@ -136,10 +136,10 @@ template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out,
     }
     store_turned(out, p, row, col, patch, v);
 }
-template <int NC> __device__ __forceinline__ void store_as(void* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
-    if (p.out_type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
-    else if (p.out_type == ZC_F16) store_rows(static_cast<__half*>(out), map, p, row, col, patch, v);
-    else if constexpr (NC >= 64) store_rows(static_cast<float*>(out), map, p, row, col, patch, v);      // (16-bit operands have 16-bit results)
+template <int NC> __device__ __forceinline__ void store_as(void* out, int type, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    if (type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
+    else if (type == ZC_F16) store_rows(static_cast<__half*>(out), map, p, row, col, patch, v);
+    else store_rows(static_cast<float*>(out), map, p, row, col, patch, v);
 }
 // The quotient by the fast reciprocal (2 ulp): with the rounded division the epilogue of a gated tile took 26,000 clocks, more than the products
 // of 3,300 k. A denominator beyond 2^126 gives 0, which is silu's limit there.
@@ -323,13 +323,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             }
             if constexpr (GATED) {
                 if (p.g) {
-                    store_as(p.g, &maps.o[1], p, row, col, patch, v);
-                    store_as(p.u, &maps.o[2], p, row, col, patch, w);
+                    store_as(p.g, p.saved_type, &maps.o[1], p, row, col, patch, v);
+                    store_as(p.u, p.saved_type, &maps.o[2], p, row, col, patch, w);
                 }
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = silu(v[i]) * w[i];
             }
-            store_as(c.z ? p.out[1] : p.out[0], &maps.o[c.z], p, row, col, patch, v);
+            store_as(c.z ? p.out[1] : p.out[0], p.out_type, &maps.o[c.z], p, row, col, patch, v);
         }
         if (lane == 0) tma_store_done();
         __syncwarp();
@@ -357,13 +357,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     }
                     if constexpr (GATED) {
                         if (p.g) {
-                            store_turned_as(p.g, p, row, c.n0 + j, patch, v);
-                            store_turned_as(p.u, p, row, c.n0 + j, patch, w);
+                            store_turned_as(p.g, p.saved_type, p, row, c.n0 + j, patch, v);
+                            store_turned_as(p.u, p.saved_type, p, row, c.n0 + j, patch, w);
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = silu(v[i]) * w[i];
                     }
-                    store_turned_as(c.z ? p.out[1] : p.out[0], p, row, c.n0 + j, patch, v);
+                    store_turned_as(c.z ? p.out[1] : p.out[0], p.out_type, p, row, c.n0 + j, patch, v);
                 }
             }
             __syncwarp();
@@ -410,7 +410,7 @@ struct FewPlan {
     bool x_vec, out_vec;                // rows of x and of the output are aligned
     void *out, *g, *u;
     uint64_t ldo;
-    int out_type;
+    int out_type, saved_type;
 };
 
 __device__ __forceinline__ void store_one(void* out, int type, uint64_t at, float v) {
@@ -420,7 +420,7 @@ __device__ __forceinline__ void store_one(void* out, int type, uint64_t at, floa
 }
 template <bool GATED> __device__ __forceinline__ void few_store(const FewPlan& p, uint64_t at, float a, float b) {
     if constexpr (GATED) {
-        if (p.g) { store_one(p.g, p.out_type, at, a); store_one(p.u, p.out_type, at, b); }
+        if (p.g) { store_one(p.g, p.saved_type, at, a); store_one(p.u, p.saved_type, at, b); }
         a = silu(a) * b;
     }
     store_one(p.out, p.out_type, at, a);
@@ -438,17 +438,17 @@ template <typename T> __device__ __forceinline__ void store_four(void* out, uint
             if (j < valid) to[j] = w[j];
     }
 }
-__device__ __forceinline__ void store_four_as(void* out, const FewPlan& p, uint64_t at, uint32_t valid, const float4& v) {
-    if (p.out_type == ZC_BF16) store_four<__nv_bfloat16>(out, at, valid, p.out_vec, v);
-    else if (p.out_type == ZC_F16) store_four<__half>(out, at, valid, p.out_vec, v);
+__device__ __forceinline__ void store_four_as(void* out, int type, const FewPlan& p, uint64_t at, uint32_t valid, const float4& v) {
+    if (type == ZC_BF16) store_four<__nv_bfloat16>(out, at, valid, p.out_vec, v);
+    else if (type == ZC_F16) store_four<__half>(out, at, valid, p.out_vec, v);
     else store_four<float>(out, at, valid, p.out_vec, v);
 }
 template <bool GATED> __device__ __forceinline__ void few_store4(const FewPlan& p, uint64_t at, uint32_t valid, float4 a, const float4& b) {
     if constexpr (GATED) {
-        if (p.g) { store_four_as(p.g, p, at, valid, a); store_four_as(p.u, p, at, valid, b); }
+        if (p.g) { store_four_as(p.g, p.saved_type, p, at, valid, a); store_four_as(p.u, p.saved_type, p, at, valid, b); }
         a = make_float4(silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w);
     }
-    store_four_as(p.out, p, at, valid, a);
+    store_four_as(p.out, p.out_type, p, at, valid, a);
 }
 __device__ __forceinline__ float4 load_peer(uint32_t addr, uint32_t rank) {
     float4 v;
@@ -677,23 +677,24 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
 }
 
-// dg = dh u s (1 + g (1 - s)), du = dh g s; eight values a thread. Bound by memory: three reads and two writes of 16 bits a value.
-template <typename T> __global__ void __launch_bounds__(256) gated_gradient_kernel(const T* __restrict__ dh, uint64_t dh_ld, const T* __restrict__ g, const T* __restrict__ u, uint32_t tokens,
-                                                                                   uint32_t ffn, T* __restrict__ dg, T* __restrict__ du) {
+// dg = dh u s (1 + g (1 - s)), du = dh g s; eight values a thread. Bound by memory: 14 bytes a value with g and u in FP32, 10 with 16 bits.
+template <typename T, typename S> __global__ void __launch_bounds__(256) gated_gradient_kernel(const T* __restrict__ dh, uint64_t dh_ld, const S* __restrict__ g, const S* __restrict__ u,
+                                                                                               uint32_t tokens, uint32_t ffn, T* __restrict__ dg, T* __restrict__ du) {
     const uint32_t per_row = ffn / 8;
     pdl_wait();
     pdl_launch_dependents();
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(tokens) * per_row; i += uint64_t(gridDim.x) * 256) {
         const uint64_t row = i / per_row, col = i % per_row;
-        alignas(16) T a[8], b[8], c[8], d[8], e[8];
-        *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(dh + row * dh_ld) + col);
-        *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(g) + i);
-        *reinterpret_cast<uint4*>(c) = __ldg(reinterpret_cast<const uint4*>(u) + i);
+        float a[8], b[8], c[8];
+        alignas(16) T d[8], e[8];
+        load8<T, true>(dh + row * dh_ld + col * 8, a);
+        load8<S, true>(g + i * 8, b);
+        load8<S, true>(u + i * 8, c);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float gv = float(b[j]), s = __fdividef(1.0f, 1.0f + __expf(-gv)), dv = float(a[j]);
-            d[j] = from_f32<T>(dv * float(c[j]) * s * (1.0f + gv * (1.0f - s)));
-            e[j] = from_f32<T>(dv * gv * s);
+            const float s = __fdividef(1.0f, 1.0f + __expf(-b[j]));
+            d[j] = from_f32<T>(a[j] * c[j] * s * (1.0f + b[j] * (1.0f - s)));
+            e[j] = from_f32<T>(a[j] * b[j] * s);
         }
         reinterpret_cast<uint4*>(dg)[i] = *reinterpret_cast<const uint4*>(d);
         reinterpret_cast<uint4*>(du)[i] = *reinterpret_cast<const uint4*>(e);
@@ -761,10 +762,10 @@ int current_device(Device& d) {
 
 int no_maps() { return fail(nullptr, ZC_EEXEC, "the driver did not encode a tensor map"); }
 // The output in boxes of 32 rows x 128 bytes, or of what a warp has of a row.
-bool map_output(CUtensorMap& m, void* out, const TilePlan& p, uint32_t columns) {
+bool map_output(CUtensorMap& m, void* out, int type, const TilePlan& p, uint32_t columns) {
     const Encode encode = tensor_map_encoder();
     if (!encode) return false;
-    const uint32_t elem_bytes = uint32_t(dtype_bytes(p.out_type)), most = 128 / elem_bytes;
+    const uint32_t elem_bytes = uint32_t(dtype_bytes(type)), most = 128 / elem_bytes;
     const cuuint64_t dims[2] = {p.N, p.M}, strides[1] = {p.ldo * elem_bytes};
     const cuuint32_t box[2] = {columns < most ? columns : most, 32}, elem[2] = {1, 1};
     return encode(&m, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, out, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -804,7 +805,7 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     // A TMA store writes whole 16-byte pieces: rows start and end on one (the other outputs are contiguous and aligned wherever they are given).
     p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && p.N * dtype_bytes(p.out_type) % 16 == 0;
     for (int i = 0; i < 3 && p.aligned; ++i)
-        if (to[i] && !map_output(maps.o[i], to[i], p, GATED ? N / 4 : N / 2)) return no_maps();
+        if (to[i] && !map_output(maps.o[i], to[i], p.g && i ? p.saved_type : p.out_type, p, GATED ? N / 4 : N / 2)) return no_maps();
     const uint32_t pairs = d.sms / 2, total = p.segs * p.kblocks;
     // K is shared by two or four pairs where all of the tiles still run at once: dx of 300 x 2048 x 8192 58 -> 39 us; MX4 256 x 2048 x 8192 10.8 us
     // with two pairs a tile, 17.5 with four, whose sixteen clusters do not all fit.
@@ -941,6 +942,12 @@ int check_gated(const char* who, int dtype, uint32_t hidden, uint32_t ffn) {
         return fail(nullptr, ZC_EINVAL, std::string(who) + ": hidden and ffn must be multiples of 8, from 8 to 1048576");
     return ZC_OK;
 }
+// g and u: where the operands' type or FP32.
+int check_saved(const char* who, const void* g, const void* u, int dtype, int saved_dtype) {
+    if (saved_dtype != dtype && saved_dtype != ZC_F32) return fail(nullptr, ZC_EINVAL, std::string(who) + ": g and u must be F32 or of the operands' dtype");
+    if (misaligned(g) || misaligned(u)) return fail(nullptr, ZC_EINVAL, std::string(who) + ": buffers must be 16-byte aligned");
+    return ZC_OK;
+}
 
 }  // namespace
 }  // namespace zc
@@ -962,17 +969,17 @@ int zc_mx4_gated(const void* x, int x_dtype, uint64_t x_ld, void* x_codes, void*
 }
 
 int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void* up, int dtype, uint32_t tokens, uint32_t hidden, uint32_t ffn, void* h, void* g, void* u,
-                     void* stream) {
+                     int saved_dtype, void* stream) {
     const char* who = "zc_gated_forward";
     int rc = check_gated(who, dtype, hidden, ffn);
     if (rc == ZC_OK) rc = check_matrix(who, x, dtype, tokens, hidden, x_ld, true);
     for (const void* w : {gate, up}) if (rc == ZC_OK) rc = check_matrix(who, w, dtype, ffn, hidden, hidden, true);
     if (rc == ZC_OK) rc = check_matrix(who, h, dtype, tokens, ffn, ffn, true);
     if (rc == ZC_OK && tokens && !g != !u) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": g and u go together");
-    for (const void* v : {g, u}) if (rc == ZC_OK && v) rc = check_matrix(who, v, dtype, tokens, ffn, ffn, true);
+    if (rc == ZC_OK && (g || u)) rc = check_saved(who, g, u, dtype, saved_dtype);
     if (rc != ZC_OK || !tokens) return rc;
-    const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2;
-    const Span in[3] = {{x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}}, to[3] = {{h, tf}, {g, tf}, {u, tf}};
+    const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2, ts = uint64_t(tokens) * ffn * dtype_bytes(saved_dtype);
+    const Span in[3] = {{x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}}, to[3] = {{h, tf}, {g, ts}, {u, ts}};
     for (int i = 0; i < 3; ++i) {
         for (const Span& v : in) if (overlap(to[i], v)) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
         for (int j = 0; j < i; ++j) if (overlap(to[i], to[j])) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
@@ -989,12 +996,12 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
         if (!map_rows(maps.a[0], gate, ffn, hidden, hidden, TILE_M) || !map_rows(maps.a[1], up, ffn, hidden, hidden, TILE_M) || !map_rows(maps.b[0], x, tokens, hidden, x_ld, p.n))
             return no_maps();
         p.idesc = idesc_f16(dtype, false, false, TILE_M, p.n);
-        p.out = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
+        p.out = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype; p.saved_type = saved_dtype;
         return launch_few<false, false, 2>(maps, p, d, s);
     }
     TilePlan p{};
     p.M = tokens; p.N = ffn; p.segs = 1; p.outs = 1;
-    p.out[0] = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype;
+    p.out[0] = h; p.g = g; p.u = u; p.ldo = ffn; p.out_type = dtype; p.saved_type = saved_dtype;
     const bool narrow = narrow_tiles(p, d, 2);
     set_tile_k(p, hidden, 64, narrow);
     const uint32_t n = narrow ? 128 : 256;
@@ -1004,7 +1011,7 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
     return narrow ? launch_tiles<false, false, false, true, 128>(maps, p, d, s) : launch_tiles<false, false, false, true, 256>(maps, p, d, s);
 }
 
-int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_ld, const void* gate, const void* up, const void* g, const void* u, int dtype, uint32_t tokens,
+int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_ld, const void* gate, const void* up, const void* g, const void* u, int saved_dtype, int dtype, uint32_t tokens,
                       uint32_t hidden, uint32_t ffn, void* dg, void* du, void* dx, void* dgate, void* dup, void* stream) {
     const char* who = "zc_gated_backward";
     int rc = check_gated(who, dtype, hidden, ffn);
@@ -1012,12 +1019,13 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     if (rc == ZC_OK) rc = check_matrix(who, x, dtype, tokens, hidden, x_ld, true);
     for (const void* w : {gate, up}) if (rc == ZC_OK) rc = check_matrix(who, w, dtype, ffn, hidden, hidden, true);
     for (const void* v : {g, u, static_cast<const void*>(dg), static_cast<const void*>(du)}) if (rc == ZC_OK) rc = check_matrix(who, v, dtype, tokens, ffn, ffn, true);
+    if (rc == ZC_OK) rc = check_saved(who, g, u, dtype, saved_dtype);
     if (rc == ZC_OK && dx) rc = check_matrix(who, dx, dtype, tokens, hidden, hidden, true);
     if (rc == ZC_OK && !dgate != !dup) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": dgate and dup go together");
     for (const void* v : {dgate, dup}) if (rc == ZC_OK && v) rc = check_matrix(who, v, dtype, ffn, hidden, hidden, true);
     if (rc != ZC_OK) return rc;
-    const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2, th = uint64_t(tokens) * hidden * 2;
-    const Span in[6] = {{dh, matrix_bytes(dtype, tokens, ffn, dh_ld)}, {x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}, {g, tf}, {u, tf}};
+    const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2, th = uint64_t(tokens) * hidden * 2, ts = uint64_t(tokens) * ffn * dtype_bytes(saved_dtype);
+    const Span in[6] = {{dh, matrix_bytes(dtype, tokens, ffn, dh_ld)}, {x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}, {g, ts}, {u, ts}};
     const Span to[5] = {{dg, tf}, {du, tf}, {dx, th}, {dgate, fh}, {dup, fh}};
     for (int i = 0; i < 5; ++i) {
         for (const Span& v : in) if (overlap(to[i], v)) return fail(nullptr, ZC_EINVAL, std::string(who) + ": overlapping buffers");
@@ -1033,11 +1041,15 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     }
     const uint64_t blocks = (uint64_t(tokens) * (ffn / 8) + 255) / 256;
     const uint32_t grid = uint32_t(blocks < 148 * 16 ? blocks : 148 * 16);
-    const auto gradient = [&](auto kernel, auto type) {
+    const auto gradient = [&](auto type, auto saved) {
         typedef decltype(type) T;
-        return launch_after(kernel, dim3(grid), 256, 0, 1, s, static_cast<const T*>(dh), dh_ld, static_cast<const T*>(g), static_cast<const T*>(u), tokens, ffn, static_cast<T*>(dg), static_cast<T*>(du));
+        typedef decltype(saved) S;
+        return launch_after(gated_gradient_kernel<T, S>, dim3(grid), 256, 0, 1, s, static_cast<const T*>(dh), dh_ld, static_cast<const S*>(g), static_cast<const S*>(u), tokens, ffn,
+                            static_cast<T*>(dg), static_cast<T*>(du));
     };
-    rc = launched(dtype == ZC_BF16 ? gradient(gated_gradient_kernel<__nv_bfloat16>, __nv_bfloat16()) : gradient(gated_gradient_kernel<__half>, __half()), "gated gradient");
+    const bool full = saved_dtype == ZC_F32;
+    rc = launched(dtype == ZC_BF16 ? (full ? gradient(__nv_bfloat16(), float()) : gradient(__nv_bfloat16(), __nv_bfloat16()))
+                                   : (full ? gradient(__half(), float()) : gradient(__half(), __half())), "gated gradient");
     if (rc != ZC_OK) return rc;
     Device d;
     if ((rc = current_device(d)) != ZC_OK) return rc;
