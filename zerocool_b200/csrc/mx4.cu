@@ -9,10 +9,11 @@ namespace zc {
 namespace {
 
 constexpr int QT_ROWS = 128, QT_COLS = 256;     // one CTA: a row of two scale tiles
+constexpr int FLIGHT = 4;                       // rows of a warp whose loads are in flight
 
 // A CTA takes 128 rows x 256 columns, so that it writes whole scale tiles (gathered in shared memory; bytes past the last row or
 // column are written 0). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of the 256, a warp walks its 16 rows
-// four at a time (four independent 16-byte loads in flight per lane for 16-bit values, eight for FP32).
+// FLIGHT at a time.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t cols, uint64_t ld,
                                                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ __align__(16) uint8_t tile[2][512];
@@ -23,17 +24,17 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
-    for (uint32_t r0 = warp * 4; r0 < n; r0 += 32) {
-        float v[4][8];
+    for (uint32_t r0 = warp * FLIGHT; r0 < n; r0 += 8 * FLIGHT) {
+        float v[FLIGHT][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < FLIGHT; ++i) {
             const bool live = r0 + i < n && col < cols;      // cols is a multiple of 32: the four lanes of a block agree
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
             if (live) load8<T, VEC>(x + uint64_t(row0 + r0 + i) * ld + col, v[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < FLIGHT; ++i) {
             uint32_t top = 0;                                // magnitudes as integers: ordered like the values, NaN above all
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
@@ -54,30 +55,42 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_
         reinterpret_cast<uint4*>(scales + (uint64_t(blockIdx.x) * tiles + t) * 512)[threadIdx.x & 31] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
 }
 
-// Eight values per thread.
+// The same shape the other way: 128 rows x 256 columns a CTA, eight columns a lane.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows,
                                                                                         uint32_t cols, T* __restrict__ out, uint64_t ld) {
-    const uint32_t per_row = cols / 8;
+    const uint32_t row0 = blockIdx.x * QT_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * QT_COLS + lane * 8;
+    const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
+    const uint8_t* const tile = scales + mx4_scale_at(row0, col / 32, (cols + 127) / 128);      // of row 0 of the 128
     pdl_wait();
     pdl_launch_dependents();
-    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(rows) * per_row; i += uint64_t(gridDim.x) * 256) {
-        const uint32_t row = uint32_t(i / per_row), col = uint32_t(i % per_row) * 8, block = col / 32;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
-        const float f = mx4_factor(__ldg(scales + mx4_scale_at(row, block, (cols + 127) / 128)));
-        T v[8];
+    if (col >= cols) return;
+    for (uint32_t r0 = warp * FLIGHT; r0 < n; r0 += 8 * FLIGHT) {
+        uint32_t word[FLIGHT], s[FLIGHT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 p = mx4_values2((word >> (8 * j)) & 0xffu);
-            v[2 * j] = from_f32<T>(p.x * f);
-            v[2 * j + 1] = from_f32<T>(p.y * f);
+        for (int i = 0; i < FLIGHT; ++i) {
+            const uint32_t r = min(r0 + i, n - 1);
+            word[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + uint64_t(row0 + r) * (cols >> 1) + (col >> 1)));
+            s[i] = __ldg(tile + (r & 31) * 16 + (r >> 5) * 4);
         }
-        T* to = out + uint64_t(row) * ld + col;
-        if constexpr (VEC) {
 #pragma unroll
-            for (uint32_t j = 0; j < sizeof(T) * 8 / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
-        } else {
+        for (int i = 0; i < FLIGHT; ++i) {
+            if (r0 + i >= n) break;
+            const float f = mx4_factor(s[i]);
+            alignas(16) T v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) to[j] = v[j];
+            for (int j = 0; j < 4; ++j) {
+                const float2 p = mx4_values2((word[i] >> (8 * j)) & 0xffu);
+                v[2 * j] = from_f32<T>(p.x * f);
+                v[2 * j + 1] = from_f32<T>(p.y * f);
+            }
+            T* to = out + uint64_t(row0 + r0 + i) * ld + col;
+            if constexpr (VEC) {
+#pragma unroll
+                for (uint32_t j = 0; j < sizeof(T) * 8 / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) to[j] = v[j];
+            }
         }
     }
 }
@@ -98,10 +111,9 @@ template <typename T> int quantize_as(const void* x, uint32_t rows, uint32_t col
     return launched(launch_after(kernel, grid, 256, 0, 1, s, static_cast<const T*>(x), rows, cols, ld, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)), "mx4 quantisation");
 }
 template <typename T> int dequantize_as(const void* codes, const void* scales, uint32_t rows, uint32_t cols, void* out, uint64_t ld, cudaStream_t s) {
-    const uint64_t blocks = (uint64_t(rows) * (cols / 8) + 255) / 256;
-    const uint32_t grid = uint32_t(blocks < 148 * 32 ? blocks : 148 * 32);
+    const dim3 grid((rows + QT_ROWS - 1) / QT_ROWS, (cols + QT_COLS - 1) / QT_COLS);
     auto kernel = rows16(out, ld, sizeof(T)) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
-    return launched(launch_after(kernel, dim3(grid), 256, 0, 1, s, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, static_cast<T*>(out), ld), "mx4 dequantisation");
+    return launched(launch_after(kernel, grid, 256, 0, 1, s, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, static_cast<T*>(out), ld), "mx4 dequantisation");
 }
 
 }  // namespace
