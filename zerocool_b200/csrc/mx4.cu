@@ -8,89 +8,75 @@
 namespace zc {
 namespace {
 
-constexpr int QT_ROWS = 128, QT_COLS = 256;     // one CTA: a row of two scale tiles
-constexpr int FLIGHT = 4;                       // rows of a warp whose loads are in flight
+constexpr int QT_ROWS = 32, QT_COLS = 256;      // one CTA: a quarter (every fourth word) of two scale tiles
+constexpr int FLIGHT = 4;                       // rows of a warp, all of their loads in flight
 
-// A CTA takes 128 rows x 256 columns, so that it writes whole scale tiles (gathered in shared memory; bytes past the last row or
-// column are written 0). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of the 256, a warp walks its 16 rows
-// FLIGHT at a time.
+// A CTA takes 32 rows x 256 columns, whose scales are every fourth 32-bit word of two tiles (gathered in shared memory; words of rows and
+// columns past the last one are written 0, so the grid covers whole tiles). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of
+// the 256, a warp its four rows at once.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t cols, uint64_t ld,
                                                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    __shared__ __align__(16) uint8_t tile[2][512];
-    const uint32_t row0 = blockIdx.x * QT_ROWS, col0 = blockIdx.y * QT_COLS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t col = col0 + lane * 8;
-    if (threadIdx.x < 64) reinterpret_cast<uint4*>(tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+    __shared__ uint32_t words[2][QT_ROWS];
+    const uint32_t row0 = blockIdx.x * QT_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * QT_COLS + lane * 8;
+    const uint32_t r0 = row0 + warp * FLIGHT;
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
-    for (uint32_t r0 = warp * FLIGHT; r0 < n; r0 += 8 * FLIGHT) {
-        float v[FLIGHT][8];
+    float v[FLIGHT][8];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            const bool live = r0 + i < n && col < cols;      // cols is a multiple of 32: the four lanes of a block agree
+    for (int i = 0; i < FLIGHT; ++i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-            if (live) load8<T, VEC>(x + uint64_t(row0 + r0 + i) * ld + col, v[i]);
-        }
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (r0 + i < rows && col < cols) load8<T, VEC>(x + uint64_t(r0 + i) * ld + col, v[i]);      // cols is a multiple of 32: the four lanes of a block agree
+    }
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            uint32_t top = 0;                                // magnitudes as integers: ordered like the values, NaN above all
+    for (int i = 0; i < FLIGHT; ++i) {
+        uint32_t top = 0;                                // magnitudes as integers: ordered like the values, NaN above all
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t s = mx4_scale(top);
-            const uint32_t word = mx4_codes8(v[i], s);
-            if (r0 + i < n && col < cols) {
-                const uint32_t r = r0 + i;
-                *reinterpret_cast<uint32_t*>(codes + uint64_t(row0 + r) * (cols >> 1) + (col >> 1)) = word;
-                if ((lane & 3) == 0) tile[lane >> 4][(r & 31) * 16 + (r >> 5) * 4 + ((lane >> 2) & 3)] = uint8_t(s);
-            }
-        }
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t s = mx4_scale(top);               // 0 where there is nothing
+        if (r0 + i < rows && col < cols) *reinterpret_cast<uint32_t*>(codes + uint64_t(r0 + i) * (cols >> 1) + (col >> 1)) = mx4_codes8(v[i], s);
+        if ((lane & 3) == 0) reinterpret_cast<uint8_t*>(&words[lane >> 4][warp * FLIGHT + i])[(lane >> 2) & 3] = uint8_t(s);
     }
     __syncthreads();
     const uint32_t tiles = (cols + 127) / 128, t = blockIdx.y * 2 + (threadIdx.x >> 5);
     if (threadIdx.x < 64 && t < tiles)
-        reinterpret_cast<uint4*>(scales + (uint64_t(blockIdx.x) * tiles + t) * 512)[threadIdx.x & 31] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+        *reinterpret_cast<uint32_t*>(scales + (uint64_t(row0 / 128) * tiles + t) * 512 + (threadIdx.x & 31) * 16 + (row0 % 128) / 32 * 4) = words[threadIdx.x >> 5][threadIdx.x & 31];
 }
 
-// The same shape the other way: 128 rows x 256 columns a CTA, eight columns a lane.
+// The same shape the other way: 32 rows x 256 columns a CTA, eight columns a lane.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows,
                                                                                         uint32_t cols, T* __restrict__ out, uint64_t ld) {
-    const uint32_t row0 = blockIdx.x * QT_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * QT_COLS + lane * 8;
-    const uint32_t n = min(uint32_t(QT_ROWS), rows - row0);
-    const uint8_t* const tile = scales + mx4_scale_at(row0, col / 32, (cols + 127) / 128);      // of row 0 of the 128
+    const uint32_t lane = threadIdx.x & 31, r0 = blockIdx.x * QT_ROWS + (threadIdx.x >> 5) * FLIGHT, col = blockIdx.y * QT_COLS + lane * 8;
     pdl_wait();
     pdl_launch_dependents();
-    if (col >= cols) return;
-    for (uint32_t r0 = warp * FLIGHT; r0 < n; r0 += 8 * FLIGHT) {
-        uint32_t word[FLIGHT], s[FLIGHT];
+    if (col >= cols || r0 >= rows) return;
+    uint32_t word[FLIGHT], s[FLIGHT];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            const uint32_t r = min(r0 + i, n - 1);
-            word[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + uint64_t(row0 + r) * (cols >> 1) + (col >> 1)));
-            s[i] = __ldg(tile + (r & 31) * 16 + (r >> 5) * 4);
+    for (int i = 0; i < FLIGHT; ++i) {
+        const uint32_t r = min(r0 + i, rows - 1);
+        word[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + uint64_t(r) * (cols >> 1) + (col >> 1)));
+        s[i] = __ldg(scales + mx4_scale_at(r, col / 32, (cols + 127) / 128));
+    }
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i) {
+        if (r0 + i >= rows) break;
+        const float f = mx4_factor(s[i]);
+        alignas(16) T v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 p = mx4_values2((word[i] >> (8 * j)) & 0xffu);
+            v[2 * j] = from_f32<T>(p.x * f);
+            v[2 * j + 1] = from_f32<T>(p.y * f);
         }
+        T* to = out + uint64_t(r0 + i) * ld + col;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            if (r0 + i >= n) break;
-            const float f = mx4_factor(s[i]);
-            alignas(16) T v[8];
+            for (uint32_t j = 0; j < sizeof(T) * 8 / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 p = mx4_values2((word[i] >> (8 * j)) & 0xffu);
-                v[2 * j] = from_f32<T>(p.x * f);
-                v[2 * j + 1] = from_f32<T>(p.y * f);
-            }
-            T* to = out + uint64_t(row0 + r0 + i) * ld + col;
-            if constexpr (VEC) {
-#pragma unroll
-                for (uint32_t j = 0; j < sizeof(T) * 8 / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) to[j] = v[j];
-            }
+            for (int j = 0; j < 8; ++j) to[j] = v[j];
         }
     }
 }
@@ -106,7 +92,7 @@ __global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restr
 }
 
 template <typename T> int quantize_as(const void* x, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, cudaStream_t s) {
-    const dim3 grid((rows + QT_ROWS - 1) / QT_ROWS, (cols + QT_COLS - 1) / QT_COLS);
+    const dim3 grid((rows + 127) / 128 * (128 / QT_ROWS), (cols + QT_COLS - 1) / QT_COLS);      // whole tiles
     auto kernel = rows16(x, ld, sizeof(T)) ? quantize_kernel<T, true> : quantize_kernel<T, false>;
     return launched(launch_after(kernel, grid, 256, 0, 1, s, static_cast<const T*>(x), rows, cols, ld, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)), "mx4 quantisation");
 }
