@@ -516,6 +516,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 } else {
                     prefetch_2d(&maps.a[i], kb * KB, m0);
                 }
+                if constexpr (MX4) prefetch_bulk(p.sfw[i] + (uint64_t(m0 / 128) * p.ktiles + kb * 2) * 512, min(2u, p.ktiles - kb * 2) * 512);
             }
         }
     }
