@@ -247,12 +247,12 @@ def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
     _same_device(x.device, dh=dh, gate=gate, up=up, g=g, u=u)
     if not input_grad and not weight_grads:
         return None, None, None
-    dg, du = torch.empty_like(g, dtype=x.dtype), torch.empty_like(u, dtype=x.dtype)
+    scratch = torch.empty((2, tokens, ffn), dtype=x.dtype, device=x.device)      # dg, du
     dx = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device) if input_grad else None
     dgate, dup = (torch.empty_like(gate), torch.empty_like(up)) if weight_grads else (None, None)
     pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     _call(x.device, "zc_gated_backward", dh.data_ptr(), dh_ld, x.data_ptr(), x_ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), CODES[saved], code,
-          tokens, hidden, ffn, dg.data_ptr(), du.data_ptr(), pointer(dx), pointer(dgate), pointer(dup))
+          tokens, hidden, ffn, scratch.data_ptr(), scratch.data_ptr() + tokens * ffn * 2, pointer(dx), pointer(dgate), pointer(dup))
     return dx, dgate, dup
 
 
