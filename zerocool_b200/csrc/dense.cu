@@ -58,11 +58,24 @@ constexpr uint32_t SPLIT_STAGES = 3;                       // stages of K that a
 
 struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
+// Division of n < 2^31 by a divisor known on the host: (umulhi(mul, n) + n) >> shift with mul = 2^32 (2^shift - d) / d + 1, 2^shift >= d. The tile
+// of an index takes two; as divisions they stopped the copying thread for 1,000 clocks a tile.
+struct Divisor {
+    uint32_t d, mul, shift;
+    void set(uint32_t by) {
+        d = by;
+        for (shift = 0; (1ull << shift) < d; ++shift) {}
+        mul = uint32_t((((1ull << shift) - d) << 32) / d + 1);
+    }
+};
+__device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor& by) { return (__umulhi(by.mul, n) + n) >> by.shift; }
+
 struct TilePlan {
     uint32_t M, N;                      // rows and columns of an output (gated: N = ffn)
     uint32_t kblocks, ksteps;           // stages of K; steps of 32 bytes in the last one
     uint32_t segs, outs;                // pairs (a[s], b[s]) whose products add up; outputs a[z] . b[0]
     uint32_t mtiles, ntiles, tiles;     // of 256 rows
+    Divisor band, last;                 // tiles of a band of eight row tiles; row tiles of the last, shorter band
     uint32_t splits, kown;              // pairs that share a tile's K (then a cluster has one tile), stages of each
     uint32_t idesc;
     uint32_t ktiles;                    // MX4: scale tiles along K
@@ -77,9 +90,11 @@ struct Tile { uint32_t z, m0, n0; };
 
 // Bands of eight row tiles, walked column by column: what runs at one time shares few rows of A and of B in L2.
 __device__ __forceinline__ Tile tile_at(const TilePlan& p, uint32_t t, uint32_t width) {
-    const uint32_t per = p.mtiles * p.ntiles, z = t / per, i = t % per, band = i / (8 * p.ntiles), j = i % (8 * p.ntiles);
-    const uint32_t rows = min(8u, p.mtiles - band * 8);
-    return {z, (band * 8 + j % rows) * 2 * TILE_M, j / rows * width};
+    const uint32_t per = p.mtiles * p.ntiles, z = t >= per, i = z ? t - per : t;      // (at most two outputs)
+    const uint32_t band = quotient(i, p.band), j = i - band * p.band.d;
+    const bool whole = band * 8 + 8 <= p.mtiles;
+    const uint32_t column = whole ? j >> 3 : quotient(j, p.last), row = j - column * (whole ? 8 : p.last.d);
+    return {z, (band * 8 + row) * 2 * TILE_M, column * width};
 }
 
 // A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on, turned (at most) sixteen columns at a time through shared memory, so
@@ -165,6 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     const uint32_t rank = blockIdx.x & 1, part = (blockIdx.x >> 1) % p.splits, lead = part * 2;       // lead: the leader's rank in the cluster
     const uint32_t pair = (blockIdx.x >> 1) / p.splits, pairs = (gridDim.x >> 1) / p.splits;
     const uint32_t k0 = part * p.kown, k1 = min(k0 + p.kown, p.segs * p.kblocks);                     // of the stages of all segments
+    const uint32_t seg0 = k0 / p.kblocks, kb0 = k0 - seg0 * p.kblocks;
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
     if (threadIdx.x == 0) {
@@ -193,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 const Tile c = tile_at(p, t, WIDTH);
                 const int row = c.m0 + rank * TILE_M;                                       // of A
                 const int col = GATED ? c.n0 : c.n0 + rank * (N / 2);                       // row of B (gated: the leader has gate's, the other up's)
-                uint32_t seg = k0 / p.kblocks, kb = k0 % p.kblocks;
+                uint32_t seg = seg0, kb = kb0;
                 for (uint32_t left = k1 - k0; left; --left, ++it) {
                     const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : seg];
                     const CUtensorMap* const mb = &maps.b[GATED ? rank : seg];
@@ -242,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 const uint32_t buf = n % ACC, acc = tmem + buf * N;
                 if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t more = 0, kb = k0 % p.kblocks;
+                uint32_t more = 0, kb = kb0;
                 for (uint32_t left = k1 - k0; left; --left) {
                     const uint32_t stage = ring + slot * STAGE, now = slot;
                     if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
@@ -821,6 +837,8 @@ uint32_t set_tiles(TilePlan& p, uint32_t width) {
     p.mtiles = uint32_t((uint64_t(p.M) + 2 * TILE_M - 1) / (2 * TILE_M));
     p.ntiles = (p.N + width - 1) / width;
     const uint64_t tiles = uint64_t(p.mtiles) * p.ntiles * p.outs;
+    p.band.set(p.ntiles <= 0x0fffffffu ? 8 * p.ntiles : 1);
+    p.last.set(p.mtiles % 8 ? p.mtiles % 8 : 8);
     return p.tiles = tiles > 0x7fffffffu ? 0 : uint32_t(tiles);
 }
 // Whether 128 columns a tile: where 256 leave half of the pairs without one.
