@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x & 1, part = (blockIdx.x >> 1) % p.splits, lead = part * 2;       // lead: the leader's rank in the cluster
-    const uint32_t pair = (blockIdx.x >> 1) / p.splits, pairs = (gridDim.x >> 1) / p.splits;
+    const uint32_t rank = cluster_rank() & 1, part = cluster_rank() >> 1, lead = part * 2;            // lead: the leader's rank in the cluster
+    const uint32_t pair = cluster_index(), pairs = cluster_count();
     const uint32_t k0 = part * p.kown, k1 = min(k0 + p.kown, p.segs * p.kblocks);                     // of the stages of all segments
-    const uint32_t seg0 = k0 / p.kblocks, kb0 = k0 - seg0 * p.kblocks;
+    const uint32_t seg0 = k0 >= p.kblocks, kb0 = k0 - (seg0 ? p.kblocks : 0);                         // (at most two segments)
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
     if (threadIdx.x == 0) {
@@ -505,8 +505,9 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* const ring_p = raw + (ring - smem_addr(raw));
-    const uint32_t rank = blockIdx.x % p.splits, m0 = blockIdx.x / p.splits * TILE_M;
+    const uint32_t rank = cluster_rank(), m0 = cluster_index() * TILE_M;                // (a launch without clusters has clusters of one)
     const uint32_t k0 = rank * p.kown, k1 = min(k0 + p.kown, p.kblocks * p.segs);
+    const uint32_t seg0 = k0 >= p.kblocks, kb0 = k0 - (seg0 ? p.kblocks : 0);           // (at most two segments)
     const bool fused = p.resident != 0;
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
@@ -523,8 +524,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (warp == 0 && elect_one()) {
+        uint32_t seg = seg0, kb = kb0;
         for (uint32_t k = k0; k < min(k0 + p.prefetch, k1); ++k) {
-            const uint32_t seg = k / p.kblocks, kb = k % p.kblocks;
             for (uint32_t i = 0; i < MATS; ++i) {
                 if constexpr (A_MN) {
                     prefetch_2d(&maps.a[seg], m0, kb * 64);
@@ -534,6 +535,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 }
                 if constexpr (MX4) prefetch_bulk(p.sfw[i] + (uint64_t(m0 / 128) * p.ktiles + kb * 2) * 512, min(2u, p.ktiles - kb * 2) * 512);
             }
+            if (++kb == p.kblocks) { kb = 0; ++seg; }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     if (warp == 0) {
         if (elect_one()) {
             // slot, its round, segment and block are counted, not divided for: a division a stage is what the loop would wait for
-            uint32_t it = 0, slot = 0, round = 0, seg = k0 / p.kblocks, kb = k0 % p.kblocks;
+            uint32_t it = 0, slot = 0, round = 0, seg = seg0, kb = kb0;
             const bool two = xtiles == 2 && p.tokens > 128;
             bool ok = true;
             for (uint32_t k = k0; k < k1; ++k, ++it) {
@@ -584,7 +586,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     } else if (warp == 1) {
         if (elect_one()) {
             bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status);
-            uint32_t slot = 0, phase = 0, kb = k0 % p.kblocks, more = 0;
+            uint32_t slot = 0, phase = 0, kb = kb0, more = 0;
             uint32_t quantised = ring + p.resident;
             bool ready = mbar_test(&full[0], 0);
             for (uint32_t k = k0; ok && k < k1; ++k) {
