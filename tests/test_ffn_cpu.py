@@ -59,7 +59,7 @@ def backward(dh=at(0), dh_ld=8, x=at(1), x_ld=16, gate=at(2), up=at(3), g=at(4),
 @pytest.mark.parametrize("call,why", [
     (lambda: quantize(x=None), b"missing buffer"), (lambda: quantize(codes=None), b"missing buffer"), (lambda: quantize(scales=None), b"missing buffer"),
     (lambda: quantize(cols=48, ld=48), b"multiple of 32"), (lambda: quantize(cols=0, ld=0), b"multiple of 32"), (lambda: quantize(cols=(1 << 20) + 32, ld=1 << 21), b"multiple of 32"),
-    (lambda: quantize(ld=63), b"row stride"), (lambda: quantize(dtype=7), b"dtype"), (lambda: quantize(dtype=3), b"dtype"), (lambda: quantize(rows=1 << 31), b"rows"),
+    (lambda: quantize(ld=63), b"row stride"), (lambda: quantize(ld=(1 << 30) + 1), b"row stride"), (lambda: quantize(dtype=7), b"dtype"), (lambda: quantize(dtype=3), b"dtype"), (lambda: quantize(rows=1 << 31), b"rows"),
     (lambda: quantize(codes=at(1) + 8), b"16-byte aligned"), (lambda: quantize(scales=at(2) + 4), b"16-byte aligned"), (lambda: quantize(x=at(0) + 1), b"aligned to its elements"),
     (lambda: quantize(codes=at(0) + 64), b"overlapping"), (lambda: quantize(scales=at(1) + 64), b"overlapping"),
     (lambda: linear(xc=None), b"missing buffer"), (lambda: linear(ws=None), b"missing buffer"), (lambda: linear(out=None), b"missing buffer"),

@@ -128,7 +128,7 @@ SIZES = [(1, 1, 32), (2, 128, 64), (7, 129, 96), (16, 64, 128), (17, 300, 160), 
          (255, 33, 2048), (257, 513, 320), (300, 1000, 992),
          (1, 260, 4128), (5, 300, 8192), (33, 200, 8224), (128, 140, 2080), (3, 20000, 96), (31, 2400, 1056),
          (1300, 2600, 160), (700, 4100, 416), (129, 9000, 2080),
-         (200, 300, 8224), (260, 141, 3104), (1000, 520, 6400)]
+         (200, 300, 8224), (260, 141, 3104), (1000, 520, 6400), (129, 1, 32), (300, 7, 96), (1, 7, 32), (64, 64, 64), (65, 64, 64)]
 
 
 @pytest.mark.parametrize("tokens,rows,cols", SIZES)
@@ -156,6 +156,44 @@ def test_gated4(ffn, tokens, ffn_, cols, dtype):
     slack = 1.1 * sums(xd, gd, 64) * u.abs() + ref.silu(g).abs() * sums(xd, ud, 64) + 1.1 * sums(xd, gd, 64) * sums(xd, ud, 64) + 2.0 ** -20 * (ref.silu(g) * u).abs()
     close(ffn.mx4_gated(q, gate, up, dtype), ref.silu(g) * u, slack)
     close(ffn.mx4_gated(x, gate, up, dtype), ref.silu(g) * u, slack, "plain")
+
+
+@pytest.mark.parametrize("tokens", [5, 60, 200])
+def test_what_is_not_finite_stays_in_its_row(ffn, tokens):
+    """A NaN or an infinity in one row of x, or of the weights, makes that row (column) of the result NaN and no other."""
+    x, w = randn((tokens, 320), 1), randn((150, 320), 2)
+    x[2, 5], x[4, 319], w[149, 100] = float("nan"), float("inf"), float("-inf")
+    qw = ffn.mx4_quantize(w)
+    for y in (ffn.mx4_linear(x, qw), ffn.mx4_linear(ffn.mx4_quantize(x), qw, torch.float32), ffn.mx4_gated(x, qw, qw)):
+        want = torch.zeros(tokens, 150, dtype=torch.bool, device="cuda")
+        want[2], want[4], want[:, 149] = True, True, True
+        assert torch.equal(torch.isnan(y), want)
+    x = randn((tokens, 64), 3, dtype=torch.bfloat16)
+    x[2, 5] = float("nan")
+    gate, up, dh = randn((72, 64), 4, dtype=torch.bfloat16), randn((72, 64), 5, dtype=torch.bfloat16), randn((tokens, 72), 6, dtype=torch.bfloat16)
+    h, g, u = ffn.gated_forward(x, gate, up, save=True)
+    dx, dgate, dup = ffn.gated_backward(dh, x, gate, up, g, u)
+    for y in (h, g, u, dx):
+        assert torch.isnan(y).any(1).nonzero().view(-1).tolist() == [2] and bool(torch.isnan(y[2]).all())
+    assert bool(torch.isnan(dgate).all()) and bool(torch.isnan(dup).all())
+
+
+def test_matrices_beyond_two_gigabytes_of_offsets(ffn):
+    """Offsets of x, codes and results that pass 32 bits: the last rows are those of the same rows alone."""
+    rows, cols = 1100000, 4096                    # 4.5e9 values
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = randn((300, cols), 1, dtype=torch.bfloat16)
+    q = ffn.mx4_quantize(x)
+    tail = ffn.mx4_quantize(x[-300:])
+    assert torch.equal(q.codes[-300:], tail.codes) and not q.codes[:1000].any()
+    w = ffn.mx4_quantize(randn((4096, cols), 2, 0.05))
+    want = ffn.mx4_linear(tail, w)
+    out = torch.full((rows, 4096), 3.0, dtype=torch.bfloat16, device="cuda")
+    ffn.mx4_linear(q, w, out=out)
+    assert torch.equal(out[-300:], want) and not out[1000000].any()
+    out.fill_(3.0)
+    ffn.mx4_dequantize(q, out=out)
+    assert torch.equal(out[-300:], ffn.mx4_dequantize(tail)) and not out[1000000].any()
 
 
 @pytest.mark.parametrize("tokens", [3, 40, 200])
@@ -201,7 +239,7 @@ def test_no_tokens(ffn):
 
 BLOCKS = [(1, 8, 8), (1, 64, 128), (5, 72, 136), (16, 128, 64), (33, 64, 200), (127, 136, 128), (128, 64, 256), (129, 264, 72), (200, 520, 392), (256, 128, 512), (513, 320, 264),
           (1, 2056, 1160), (9, 4096, 136), (65, 520, 4104), (128, 1032, 1032), (2, 40, 20008), (1100, 264, 2600), (1500, 2056, 136),
-          (200, 2056, 136), (130, 40, 4104), (1500, 136, 136), (900, 1032, 520)]
+          (200, 2056, 136), (130, 40, 4104), (1500, 136, 136), (900, 1032, 520), (130, 8, 8), (300, 16, 8), (64, 8, 264), (70, 264, 8)]
 
 
 @pytest.mark.parametrize("tokens,hidden,width", BLOCKS)

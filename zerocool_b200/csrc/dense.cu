@@ -37,7 +37,7 @@ int check_matrix(const char* who, const void* p, int dtype, uint32_t rows, uint3
     if (dtype != ZC_BF16 && dtype != ZC_F16 && (dtype != ZC_F32 || tma)) return bad(tma ? "dtype must be BF16 or F16" : "dtype must be BF16, F16 or F32");
     if (!cols || rows > 0x7fffffffu) return bad("invalid shape");
     if (rows > 1 && ld < cols) return bad("row stride below the row's length");
-    if (ld > (1ull << 40)) return bad("row stride above 2^40");
+    if (ld > (1ull << 30)) return bad("row stride above 2^30");
     if (!rows) return ZC_OK;
     if (!p) return bad("missing buffer");
     if (misaligned(p, tma ? 16 : dtype_bytes(dtype))) return bad(tma ? "buffers must be 16-byte aligned" : "buffer is not aligned to its elements");
