@@ -377,7 +377,9 @@ def test_python_refusals(ffn):
     for call, why in ((lambda: ffn.mx4_quantize(x.double()), "dtype"), (lambda: ffn.mx4_quantize(x[:, :40]), "multiple of 32"), (lambda: ffn.mx4_quantize(x.t()), "columns"),
                       (lambda: ffn.mx4_quantize(x[0]), "matrix"), (lambda: ffn.mx4_linear(x[:, :32].contiguous(), w), "columns"), (lambda: ffn.mx4_linear(x, w, torch.int8), "dtype"),
                       (lambda: ffn.mx4_linear(x, w, out=torch.empty(4, 9, device="cuda")), "out must be"),
-                      (lambda: ffn.mx4_gated(x, w, ffn.mx4_quantize(randn((9, 64), 2))), "differ in shape"),
+                      (lambda: ffn.mx4_gated(x, w, ffn.mx4_quantize(randn((9, 64), 2))), "differ in shape"), (lambda: ffn.mx4_linear(x, x), "must be Mx4"),
+                      (lambda: ffn.mx4_from_rows(w.codes[0], torch.zeros(8, 2, dtype=torch.uint8, device="cuda")), "codes must be"),
+                      (lambda: ffn.mx4_linear(x.cpu(), w), "CUDA"), (lambda: ffn.mx4_linear(x, w, out=torch.empty(4, 8)), "CUDA"),
                       (lambda: ffn.Mx4(w.codes[:, :8], w.scales), "codes"), (lambda: ffn.Mx4(w.codes, w.scales[:256]), "scales"),
                       (lambda: ffn.mx4_from_rows(w.codes, torch.zeros(8, 3, dtype=torch.uint8, device="cuda")), "scales"),
                       (lambda: ffn.gated_forward(x.bfloat16(), x.half(), x.half()), "gate must be"), (lambda: ffn.gated_forward(x.half(), x.half()[:, :32], x.half()), "gate must be"),

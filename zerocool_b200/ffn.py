@@ -23,6 +23,8 @@ EXPORTS = ["zc_mx4_scale_bytes", "zc_mx4_quantize", "zc_mx4_dequantize", "zc_mx4
            "zc_gated_forward", "zc_gated_backward", "zc_ffn_status"]
 
 _lib = None
+# torch's handle of the current stream without a Stream object around it (2 us less a call); absent from builds without CUDA.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def load_library():
@@ -81,8 +83,8 @@ def _same_device(device, **others):
 
 def _call(device, name, *args):
     """One library call on the device's current stream (its last argument), with that device current."""
-    lib = load_library()
-    stream = torch.cuda.current_stream(device).cuda_stream
+    lib = _lib or load_library()
+    stream = _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
     if device.index == torch.cuda.current_device():
         rc = getattr(lib, name)(*args, stream)
     else:
@@ -163,7 +165,9 @@ def mx4_dequantize(q, dtype=None, out=None):
 
 def mx4_from_rows(codes, scales):
     """A checkpoint's codes [rows, cols / 2] and row-major scales [rows, cols / 32] (both uint8) -> Mx4 (the codes are not copied)."""
-    if scales.dim() != 2 or scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], codes.shape[-1] // 16):
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError("codes must be uint8 [rows, cols / 2]")
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], codes.shape[1] // 16):
         raise ValueError("scales must be contiguous uint8 [rows, cols / 32]")
     q = Mx4(codes, torch.empty(_scale_bytes(codes.shape[0], codes.shape[1] * 2), dtype=torch.uint8, device=codes.device))
     _same_device(codes.device, scales=scales)
@@ -172,29 +176,31 @@ def mx4_from_rows(codes, scales):
 
 
 def _mx4_product(entry, x, weights, out_dtype, out):
+    for w in weights:
+        if not isinstance(w, Mx4):
+            raise ValueError("the weights must be Mx4 (mx4_quantize)")
     w = weights[0]
     device, cols, rows = w.device, w.cols, w.rows
     for other in weights[1:]:
         if (other.rows, other.cols) != (rows, cols):
             raise ValueError(f"the weights differ in shape: [{rows}, {cols}] and [{other.rows}, {other.cols}]")
-        _same_device(device, weights=other)
     if isinstance(x, Mx4):
         tokens, xcols, plain = x.rows, x.cols, (None, F32, 0)
-        q = x
+        codes, scales = x.codes.data_ptr(), x.scales.data_ptr()
     else:
         ld = _matrix("x", x)
         (tokens, xcols), plain = x.shape, (x.data_ptr(), _code(x.dtype), ld)
-        q = None
+        scratch = torch.empty(tokens * cols // 2 + _scale_bytes(tokens, cols), dtype=torch.uint8, device=device)      # codes, then scales
+        codes = scratch.data_ptr()
+        scales = codes + tokens * cols // 2
     if xcols != cols:
         raise ValueError(f"x has {xcols} columns, the weights {cols}")
-    _same_device(device, x=x)
+    _same_device(device, x=x, weights=weights[-1])
     out_dtype = out.dtype if out_dtype is None and out is not None else out_dtype or torch.bfloat16
     code = _code(out_dtype)
     out, out_ld = _out(out, tokens, rows, out_dtype, device)
-    if q is None:
-        q = Mx4.empty(tokens, cols, device)
     pointers = [p for m in weights for p in (m.codes.data_ptr(), m.scales.data_ptr())]
-    _call(device, entry, *plain, q.codes.data_ptr(), q.scales.data_ptr(), tokens, cols, *pointers, rows, out.data_ptr(), code, out_ld)
+    _call(device, entry, *plain, codes, scales, tokens, cols, *pointers, rows, out.data_ptr(), code, out_ld)
     return out
 
 
