@@ -372,6 +372,35 @@ def test_calls_on_two_streams_at_once(ffn):
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
+def test_every_kernel_beside_every_other_and_the_expert_layer(ffn):
+    """Kernels of one and of many tokens, in 4 and in 16 bits, on four streams at once, beside the routed layer's tensor-core kernels: the
+    results are those of the calls alone."""
+    from tests import util
+    from zerocool_b200.moe import Moe
+    cfg = util.cfg2(experts=32, max_tokens=512)
+    layer = Moe(cfg, 0)
+    layer.synth_fill_layer(0, 7)
+    tokens = randn((512, cfg.hidden), 9, dtype=torch.bfloat16)
+    w = [ffn.mx4_quantize(randn((1024, 2048), 20 + i, 0.05)) for i in range(2)]
+    v = [randn((1024, 2048), 30 + i, 0.05, torch.bfloat16) for i in range(2)]
+    jobs = []
+    for n in (1, 60, 64, 300, 900):
+        x = randn((n, 2048), 40 + n, dtype=torch.bfloat16)
+        jobs += [lambda x=x: ffn.mx4_linear(x, w[0]), lambda x=x: ffn.mx4_gated(x, *w), lambda x=x: ffn.gated_forward(x, *v)]
+    jobs.append(lambda: layer.prefill(0, tokens))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for round_ in range(6):
+        for i, job in enumerate(jobs[:-1]):
+            with torch.cuda.stream(streams[(i + round_) % 3]):
+                got.append((i, job()))
+        got.append((len(jobs) - 1, jobs[-1]()))            # a handle is driven by one stream
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    assert layer.status() == 0
+
+
 def test_python_refusals(ffn):
     x, w = randn((4, 64), 1), ffn.mx4_quantize(randn((8, 64), 2))
     for call, why in ((lambda: ffn.mx4_quantize(x.double()), "dtype"), (lambda: ffn.mx4_quantize(x[:, :40]), "multiple of 32"), (lambda: ffn.mx4_quantize(x.t()), "columns"),

@@ -162,9 +162,18 @@ __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + exp
 
 // A stage is `depth` blocks of K, loaded and released together: with 128 columns a block is worth 256 clocks of products, and waiting for it,
 // releasing it and going round cost the issuing thread 300 beside its products' 40 each.
+//
+// A CTA that waits for tensor memory while others wait for it could close a circle over two SMs (two clusters, each with one CTA that has its
+// columns and one that has not). So no CTA here ever waits for another's columns: each takes at least the share of its SM's shared memory that it
+// takes of the tensor memory, so that those that fit an SM together find their columns free. A tile CTA takes all 512, hence all of the shared memory.
+constexpr uint32_t SM_SMEM = 228 * 1024, CTA_RESERVED = 1024, CTA_STATIC = 256, CTA_SMEM_MAX = 227 * 1024 - CTA_STATIC;
+constexpr uint32_t smem_share(uint32_t tmem_columns) { return tmem_columns * (SM_SMEM / 512) - CTA_RESERVED - CTA_STATIC; }
+
 template <bool MX4, int N> struct TileSmem {
     static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = N == 256 ? 1 : 2, stage = depth * block;
-    static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, bytes = stages * stage + 8 * PATCH_BYTES + 1024;
+    static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, used = stages * stage + 8 * PATCH_BYTES + 1024;
+    static constexpr uint32_t bytes = smem_share(512);
+    static_assert(used <= bytes && bytes <= CTA_SMEM_MAX, "shared memory of a tile CTA");
 };
 
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
@@ -174,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     constexpr uint32_t KB = MX4 ? 128 : 64;               // TMA elements of K a block (bytes of codes, 16-bit values)
     constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;
+    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;       // (CTA_STATIC bytes at most)
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank() & 1, part = cluster_rank() >> 1, lead = part * 2;            // lead: the leader's rank in the cluster
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 constexpr uint32_t FEW_THREADS = 192, FEW_STAGES = 8;
 // 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
 constexpr uint32_t FEW_TOKENS = 64;
-constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_SMEM_MAX = 226 * 1024;      // what a ring may take (two CTAs an SM); the most a CTA may have
+constexpr uint32_t FEW_SMEM = 110 * 1024;                                 // what a ring may take (two CTAs an SM)
 // x is quantised inside up to these: MX4 8192 x 4096, 1 / 2 / 4 / 8 tokens 6.4 / 7.2 / 8.7 / 11.3 us, by a launch of its own 8.1 / 8.2 / 8.2 / 8.5.
 constexpr uint32_t FEW_PLAIN_TOKENS = 2, FEW_PLAIN_BYTES = 32 * 1024;
 constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
@@ -501,7 +510,7 @@ template <bool MX4, bool A_MN, int MATS>
 __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant__ TileMaps maps, const FewPlan p) {
     constexpr uint32_t KB = MX4 ? 128 : 64;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[FEW_STAGES], empty[FEW_STAGES], acc_full, tokens_ready, drain;
+    __shared__ uint64_t full[FEW_STAGES], empty[FEW_STAGES], acc_full, tokens_ready, drain;     // (CTA_STATIC bytes at most)
     __shared__ uint32_t tmem_s, abort_s;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* const ring_p = raw + (ring - smem_addr(raw));
@@ -886,6 +895,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.sf_columns = mx4 ? mats * 8 + 8 * xtiles : 0;
     p.tmem_columns = 32;
     while (p.tmem_columns < p.sf_column + p.stages * p.sf_columns) p.tmem_columns *= 2;
+    if (p.smem < smem_share(p.tmem_columns)) p.smem = smem_share(p.tmem_columns);
     const uint64_t ahead = FEW_AHEAD / (uint64_t(mtiles) * p.splits * mats * A_BYTES);
     p.prefetch = ahead < p.kown ? uint32_t(ahead) : p.kown;
 }
@@ -894,7 +904,7 @@ template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, Fe
     static Configured configured;
     p.out_vec = rows16(p.out, p.ldo, dtype_bytes(p.out_type));
     auto kernel = few_kernel<MX4, A_MN, MATS>;
-    const int rc = configured.once(kernel, d.index, FEW_SMEM_MAX, FEW_THREADS, false);
+    const int rc = configured.once(kernel, d.index, CTA_SMEM_MAX, FEW_THREADS, false);
     if (rc != ZC_OK) return rc;
     return launched(launch_after(kernel, dim3((p.M + TILE_M - 1) / TILE_M * p.splits), FEW_THREADS, p.smem, p.splits, s, maps, p), "dense product of few tokens");
 }
