@@ -54,8 +54,6 @@ constexpr uint32_t A_BYTES = TILE_M * 128;
 constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory columns of a stage's scales: A 2 x 4, B 2 x 8 at most
 constexpr uint32_t PATCH = 17, PATCH_BYTES = 4096;         // a warp's shared memory of the epilogue, and the floats of a row where it turns rows in it
 
-constexpr uint32_t SPLIT_STAGES = 3;                       // stages of K that a pair keeps where pairs share a tile
-
 struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
 // Division of n < 2^31 by a divisor known on the host: (umulhi(mul, n) + n) >> shift with mul = 2^32 (2^shift - d) / d + 1, 2^shift >= d. The tile
@@ -169,16 +167,17 @@ __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + exp
 constexpr uint32_t SM_SMEM = 228 * 1024, CTA_RESERVED = 1024, CTA_STATIC = 256, CTA_SMEM_MAX = 227 * 1024 - CTA_STATIC;
 constexpr uint32_t smem_share(uint32_t tmem_columns) { return tmem_columns * (SM_SMEM / 512) - CTA_RESERVED - CTA_STATIC; }
 
-template <bool MX4, int N> struct TileSmem {
+template <bool MX4, bool GATED, int N> struct TileSmem {
     static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = N == 256 ? 1 : 2, stage = depth * block;
     static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, used = stages * stage + 8 * PATCH_BYTES + 1024;
     static constexpr uint32_t bytes = smem_share(512);
+    static constexpr bool shared = N == 128 || (MX4 && GATED);      // whether pairs may share a tile's K (the others are narrow where tiles are few)
     static_assert(used <= bytes && bytes <= CTA_SMEM_MAX, "shared memory of a tile CTA");
 };
 
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const TilePlan p) {
-    typedef TileSmem<MX4, N> Smem;
+    typedef TileSmem<MX4, GATED, N> Smem;
     constexpr uint32_t STAGES = Smem::stages, STAGE = Smem::stage, DEPTH = Smem::depth, ACC = MX4 && N == 256 ? 1 : 2, SF_COLUMN = ACC * N;
     constexpr uint32_t KB = MX4 ? 128 : 64;               // TMA elements of K a block (bytes of codes, 16-bit values)
     constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive_at(map_to(smem_addr(&acc_empty[buf]), lead));
             const uint32_t row = c.m0 + rank * TILE_M + quarter * 32, col = c.n0 + half * COLS;
-            if (N == 128 && p.splits > 1) {
+            if (Smem::shared && p.splits > 1) {
                 // The sums of this part of K, [column][row]; every stage of the ring has been read.
                 float* const mine = reinterpret_cast<float*>(raw + (ring - smem_addr(raw))) + half * COLS * TILE_M + quarter * 32 + lane;
 #pragma unroll
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         if (lane == 0) tma_store_done();
         __syncwarp();
     }
-    if constexpr (N == 128) {
+    if constexpr (Smem::shared) {
         if (p.splits > 1) {
             // Every pair adds a part of the tile's columns over the pairs, in their order, eight columns a warp at a time.
             cluster_sync();
@@ -827,8 +826,8 @@ struct Configured {
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(TileMaps& maps, TilePlan& p, const Device& d, cudaStream_t s) {
     static Configured configured;
     auto kernel = tile_kernel<MX4, A_MN, B_MN, GATED, N>;
-    constexpr uint32_t smem = TileSmem<MX4, N>::bytes;
-    const int rc = configured.once(kernel, d.index, smem, THREADS, N == 128);
+    constexpr uint32_t smem = TileSmem<MX4, GATED, N>::bytes;
+    const int rc = configured.once(kernel, d.index, smem, THREADS, TileSmem<MX4, GATED, N>::shared);
     if (rc != ZC_OK) return rc;
     void* const to[3] = {p.out[0], p.g ? p.g : p.out[1], p.u};
     // A TMA store writes whole 16-byte pieces: rows start and end on one (the other outputs are contiguous and aligned wherever they are given).
@@ -836,10 +835,14 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     for (int i = 0; i < 3 && p.aligned; ++i)
         if (to[i] && !map_output(maps.o[i], to[i], p.g && i ? p.saved_type : p.out_type, p, GATED ? N / 4 : N / 2)) return no_maps();
     const uint32_t pairs = d.sms / 2, total = p.segs * p.kblocks;
-    // K is shared by two or four pairs where all of the tiles still run at once: dx of 300 x 2048 x 8192 58 -> 39 us; MX4 256 x 2048 x 8192 10.8 us
-    // with two pairs a tile, 17.5 with four, whose sixteen clusters do not all fit.
+    // K is shared by four or two pairs where all of the tiles still run at once and it is long enough to pay for the sums: narrow tiles, four pairs
+    // from 12 stages on (16-bit 256 x 2048 x 512 8.9 us, shared by none 9.9; of 8 stages 8.3 by two and 7.6), two from 18 (512 x 3000 x 1000 15.1 and
+    // 19.1; of 12 stages 10.3 and 9.4); wide ones, whose sums are twice as many, 16 (MX4 gated 300 x 4000 x 600 11.9 and 12.8) and 32
+    // (of 16 stages 13.0 and 11.1).
+    typedef TileSmem<MX4, GATED, N> Smem;
     p.splits = 1;
-    for (int i = 0; N == 128 && i < 2 && p.tiles <= configured.clusters[d.index][i] && total >= (2u << i) * SPLIT_STAGES; ++i) p.splits = 2u << i;
+    if (Smem::shared && p.tiles <= configured.clusters[d.index][1] && total >= (Smem::depth == 2 ? 12 : 16)) p.splits = 4;
+    else if (Smem::shared && p.tiles <= configured.clusters[d.index][0] && total >= (Smem::depth == 2 ? 18 : 32)) p.splits = 2;
     p.kown = (total + p.splits - 1) / p.splits;
     return launched(launch_after(kernel, dim3(2 * p.splits * (p.splits > 1 || p.tiles < pairs ? p.tiles : pairs)), THREADS, smem, 2 * p.splits, s, maps, p), "dense product");
 }
