@@ -407,15 +407,17 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // one tile of 128 weight rows (of gate and of up) and one run of blocks of K; the CTAs of a cluster share a tile's K and add their partial
 // sums through distributed shared memory, in the order of their ranks. The lanes of the epilogue hold consecutive output columns of
 // a token, so plain stores are coalesced whatever the row stride.
-// One or two plain tokens: every CTA quantises its own part of their K into shared memory (the epilogue warps, while the weights arrive),
+// A handful of plain tokens: every CTA quantises its own part of their K into shared memory (the epilogue warps, while the weights arrive),
 // in the swizzle TMA would have written (more are quantised by a launch of their own). The kernel before may still run while this one starts (programmatic launch): until it has
 // ended nothing is read but into L2, where a later write of it would arrive too.
 constexpr uint32_t FEW_THREADS = 192, FEW_STAGES = 8;
 // 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
 constexpr uint32_t FEW_TOKENS = 64;
 constexpr uint32_t FEW_SMEM = 110 * 1024;                                 // what a ring may take (two CTAs an SM)
-// x is quantised inside up to these: MX4 8192 x 4096, 1 / 2 / 4 / 8 tokens 6.4 / 7.2 / 8.7 / 11.3 us, by a launch of its own 8.1 / 8.2 / 8.2 / 8.5.
-constexpr uint32_t FEW_PLAIN_TOKENS = 2, FEW_PLAIN_BYTES = 32 * 1024;
+// x is quantised inside where a CTA has at most so many rows of 256 of its columns (tokens x blocks; the four warps share them): MX4 2048 x 512, one block a
+// CTA, 1 / 4 / 8 / 12 / 16 tokens 3.4 / 3.6 / 4.3 / 4.8 / 5.3 us, by a launch of its own 4.6 / 4.8 / 4.8 / 5.0 / 5.2; 8192 x 4096, four blocks, 2 / 3 / 4
+// tokens 7.2 / 7.7 / 8.5 and 8.2 / 8.5 / 8.6.
+constexpr uint32_t FEW_PLAIN_ROWS = 12, FEW_PLAIN_BYTES = 32 * 1024;
 constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
 
 struct FewPlan {
@@ -482,26 +484,27 @@ __device__ __forceinline__ float4 load_peer(uint32_t addr, uint32_t rank) {
 // The tokens' blocks [k0, k0 + blocks) of 256 columns into shared memory: per block n rows of 128 bytes, then two scale tiles. A warp takes a
 // row of a block at a time, eight values a lane (four lanes share a scale). Padding rows stay as they are (their columns are not stored);
 // columns past the last one become zero codes with a zero scale byte. The loop is not unrolled: a launch of a few microseconds waits for
-// its instructions too (gated block of 512 x 2048, one token: 4.1 us, with four rows in flight 4.7).
+// its instructions too (gated block of 512 x 2048, one token: 4.0 us, with four rows in flight 4.7).
 template <typename T> __device__ __forceinline__ void quantise_tokens(const FewPlan& p, uint32_t k0, uint32_t blocks, uint8_t* to) {
     const uint32_t lane = threadIdx.x & 31, size = p.n * 128 + 1024, left = p.cols - k0 * 256;
-    for (uint32_t t = 0; t < p.tokens; ++t) {
-        const T* const row = static_cast<const T*>(p.x) + uint64_t(t) * p.x_ld + uint64_t(k0) * 256;
+    const T* const x = static_cast<const T*>(p.x) + uint64_t(k0) * 256;
 #pragma unroll 1
-        for (uint32_t block = (threadIdx.x >> 5) - 2; block < blocks; block += 4) {
-            const uint32_t at = block * 256 + lane * 8;
-            float v[8] = {};
-            if (at < left) p.x_vec ? load8<T, true>(row + at, v) : load8<T, false>(row + at, v);
-            uint32_t top = 0;
+    for (uint32_t t = 0, block = (threadIdx.x >> 5) - 2;; block += 4) {       // rows of blocks, token by token, dealt to the four warps in turn
+        while (block >= blocks) { block -= blocks; ++t; }
+        if (t >= p.tokens) break;
+        const T* const row = x + uint64_t(t) * p.x_ld;
+        const uint32_t at = block * 256 + lane * 8;
+        float v[8] = {};
+        if (at < left) p.x_vec ? load8<T, true>(row + at, v) : load8<T, false>(row + at, v);
+        uint32_t top = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t s = mx4_scale(top);
-            uint8_t* const b = to + block * size;
-            *reinterpret_cast<uint32_t*>(b + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = mx4_codes8(v, s);
-            if ((lane & 3) == 0) b[p.n * 128 + (lane >> 4) * 512 + (t & 31) * 16 + (t >> 5) * 4 + ((lane >> 2) & 3)] = uint8_t(s);
-        }
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t s = mx4_scale(top);
+        uint8_t* const b = to + block * size;
+        *reinterpret_cast<uint32_t*>(b + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = mx4_codes8(v, s);
+        if ((lane & 3) == 0) b[p.n * 128 + (lane >> 4) * 512 + (t & 31) * 16 + (t >> 5) * 4 + ((lane >> 2) & 3)] = uint8_t(s);
     }
 }
 
@@ -883,7 +886,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.kown = (total + splits - 1) / splits;
     p.splits = (total + p.kown - 1) / p.kown;
     const uint32_t quantised = p.kown * (p.n * 128 + 1024), xtiles = p.n > 128 ? 2 : 1;
-    const bool fused = plain && p.tokens <= FEW_PLAIN_TOKENS && quantised <= FEW_PLAIN_BYTES;
+    const bool fused = plain && p.tokens * p.kown <= FEW_PLAIN_ROWS && quantised <= FEW_PLAIN_BYTES;
     p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? xtiles * 1024 : 0));
     const uint32_t room = FEW_SMEM - 1024 - (fused ? quantised : 0);
     p.stages = room / p.stage;
