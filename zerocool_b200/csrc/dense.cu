@@ -417,7 +417,7 @@ constexpr uint32_t FEW_SMEM = 110 * 1024;                                 // wha
 // x is quantised inside where a CTA has at most so many rows of 256 of its columns (tokens x blocks; the four warps share them): MX4 2048 x 512, one block a
 // CTA, 1 / 4 / 8 / 12 / 16 tokens 3.4 / 3.6 / 4.3 / 4.8 / 5.3 us, by a launch of its own 4.6 / 4.8 / 4.8 / 5.0 / 5.2; 8192 x 4096, four blocks, 2 / 3 / 4
 // tokens 7.2 / 7.7 / 8.5 and 8.2 / 8.5 / 8.6.
-constexpr uint32_t FEW_PLAIN_ROWS = 12, FEW_PLAIN_BYTES = 32 * 1024;
+constexpr uint32_t FEW_PLAIN_ROWS = 12;
 constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
 
 struct FewPlan {
@@ -886,7 +886,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.kown = (total + splits - 1) / splits;
     p.splits = (total + p.kown - 1) / p.kown;
     const uint32_t quantised = p.kown * (p.n * 128 + 1024), xtiles = p.n > 128 ? 2 : 1;
-    const bool fused = plain && p.tokens * p.kown <= FEW_PLAIN_ROWS && quantised <= FEW_PLAIN_BYTES;
+    const bool fused = plain && p.tokens * p.kown <= FEW_PLAIN_ROWS;
     p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? xtiles * 1024 : 0));
     const uint32_t room = FEW_SMEM - 1024 - (fused ? quantised : 0);
     p.stages = room / p.stage;
