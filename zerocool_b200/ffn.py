@@ -75,6 +75,13 @@ def _matrix(name, t, shape=None, dtype=None, contiguous=False):
     return t.stride(0) if rows > 1 else cols
 
 
+def _whole(name, t, shape, dtype, device):
+    """Checks a contiguous matrix of this shape, type and device: all at once, and one by one where that fails."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
+        _matrix(name, t, shape, dtype, contiguous=True)
+        _same_device(device, **{name: t})
+
+
 def _same_device(device, **others):
     for name, t in others.items():
         if t is not None and t.device != device:
@@ -101,8 +108,7 @@ def _scale_bytes(rows, cols):
 def _out(out, rows, cols, dtype, device, name="out"):
     """The output matrix and its row stride."""
     if out is None:
-        out = torch.empty((rows, cols), dtype=dtype, device=device)
-        return out, cols
+        return torch.empty((rows, cols), dtype=dtype, device=device), cols
     ld = _matrix(name, out, (rows, cols), dtype)
     _same_device(device, **{name: out})
     return out, ld
@@ -136,20 +142,24 @@ class Mx4:
 
     @staticmethod
     def empty(rows, cols, device):
-        return Mx4(torch.empty((rows, cols // 2), dtype=torch.uint8, device=device), torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))
+        if cols <= 0 or cols % 32:
+            raise ValueError("columns must be a multiple of 32")
+        q = object.__new__(Mx4)          # nothing to check
+        q.codes = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
+        q.scales = q.codes.new_empty(_scale_bytes(rows, cols))
+        return q
 
 
 def mx4_quantize(x, out=None):
     """x [rows, cols] (bfloat16, float16 or float32, cols a multiple of 32) -> Mx4; ``out``: an Mx4 of that shape to write."""
     ld = _matrix("x", x)
     rows, cols = x.shape
-    if not cols or cols % 32:
-        raise ValueError("columns must be a multiple of 32")
     if out is None:
         out = Mx4.empty(rows, cols, x.device)
-    elif (out.rows, out.cols) != (rows, cols):
-        raise ValueError(f"out must be [{rows}, {cols}]")
-    _same_device(x.device, out=out)
+    else:
+        if (out.rows, out.cols) != (rows, cols):
+            raise ValueError(f"out must be [{rows}, {cols}]")
+        _same_device(x.device, out=out)
     _call(x.device, "zc_mx4_quantize", x.data_ptr(), _code(x.dtype), rows, cols, ld, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
@@ -221,20 +231,19 @@ def gated_forward(x, gate, up, save=False, save_dtype=torch.float32, out=None):
     code = _code(getattr(x, "dtype", None), sixteen=True)
     ld = _matrix("x", x)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
-    for name, w in (("gate", gate), ("up", up)):
-        _matrix(name, w, (ffn, hidden), x.dtype, contiguous=True)
-    _same_device(x.device, gate=gate, up=up)
+    dtype, device = x.dtype, x.device
+    _whole("gate", gate, (ffn, hidden), dtype, device)
+    _whole("up", up, (ffn, hidden), dtype, device)
     if out is None:
-        out = torch.empty((tokens, ffn), dtype=x.dtype, device=x.device)
+        out = x.new_empty((tokens, ffn))
     else:
-        _matrix("out", out, (tokens, ffn), x.dtype, contiguous=True)
-        _same_device(x.device, out=out)
+        _whole("out", out, (tokens, ffn), dtype, device)
     g, u, saved = None, None, code
     if save:
         if save_dtype not in (torch.float32, x.dtype):
             raise ValueError(f"save_dtype must be float32 or {x.dtype}, not {save_dtype}")
         g, u, saved = torch.empty_like(out, dtype=save_dtype), torch.empty_like(out, dtype=save_dtype), CODES[save_dtype]
-    _call(x.device, "zc_gated_forward", x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), code, tokens, hidden, ffn, out.data_ptr(),
+    _call(device, "zc_gated_forward", x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), code, tokens, hidden, ffn, out.data_ptr(),
           g.data_ptr() if save else None, u.data_ptr() if save else None, saved)
     return (out, g, u) if save else out
 
@@ -244,20 +253,21 @@ def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
     code = _code(getattr(x, "dtype", None), sixteen=True)
     x_ld = _matrix("x", x)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
-    for name, w in (("gate", gate), ("up", up)):
-        _matrix(name, w, (ffn, hidden), x.dtype, contiguous=True)
-    dh_ld = _matrix("dh", dh, (tokens, ffn), x.dtype)
-    saved = torch.float32 if getattr(g, "dtype", None) == torch.float32 else x.dtype
-    for name, t in (("g", g), ("u", u)):
-        _matrix(name, t, (tokens, ffn), saved, contiguous=True)
-    _same_device(x.device, dh=dh, gate=gate, up=up, g=g, u=u)
+    dtype, device = x.dtype, x.device
+    _whole("gate", gate, (ffn, hidden), dtype, device)
+    _whole("up", up, (ffn, hidden), dtype, device)
+    dh_ld = _matrix("dh", dh, (tokens, ffn), dtype)
+    _same_device(device, dh=dh)
+    saved = torch.float32 if getattr(g, "dtype", None) == torch.float32 else dtype
+    _whole("g", g, (tokens, ffn), saved, device)
+    _whole("u", u, (tokens, ffn), saved, device)
     if not input_grad and not weight_grads:
         return None, None, None
-    scratch = torch.empty((2, tokens, ffn), dtype=x.dtype, device=x.device)      # dg, du
-    dx = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device) if input_grad else None
+    scratch = x.new_empty((2, tokens, ffn))      # dg, du
+    dx = x.new_empty((tokens, hidden)) if input_grad else None
     dgate, dup = (torch.empty_like(gate), torch.empty_like(up)) if weight_grads else (None, None)
     pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _call(x.device, "zc_gated_backward", dh.data_ptr(), dh_ld, x.data_ptr(), x_ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), CODES[saved], code,
+    _call(device, "zc_gated_backward", dh.data_ptr(), dh_ld, x.data_ptr(), x_ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), CODES[saved], code,
           tokens, hidden, ffn, scratch.data_ptr(), scratch.data_ptr() + tokens * ffn * 2, pointer(dx), pointer(dgate), pointer(dup))
     return dx, dgate, dup
 
