@@ -52,7 +52,6 @@ __device__ uint32_t ffn_status_word;     // the device's status word of these op
 constexpr uint32_t TILE_M = 128, THREADS = 320;           // rows of a CTA
 constexpr uint32_t A_BYTES = TILE_M * 128;
 constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory columns of a stage's scales: A 2 x 4, B 2 x 8 at most
-constexpr uint32_t PATCH = 17, PATCH_BYTES = 4096;         // a warp's shared memory of the epilogue, and the floats of a row where it turns rows in it
 
 struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
@@ -95,38 +94,81 @@ __device__ __forceinline__ Tile tile_at(const TilePlan& p, uint32_t t, uint32_t 
     return {z, (band * 8 + row) * 2 * TILE_M, column * width};
 }
 
-// A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on, turned (at most) sixteen columns at a time through shared memory, so
-// that as many lanes store consecutive columns; rows past the last one and columns past it are left out.
-template <typename T, int NC> __device__ __forceinline__ void store_turned(T* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
-    constexpr int TURN = NC < 16 ? NC : 16;
+// A warp's 32 rows (one a lane) of eight columns, from (row, col) of the output on, turned through shared memory, so that eight lanes store
+// consecutive columns; rows and columns past the last one are left out.
+template <typename T> __device__ __forceinline__ void store_eight(T* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[8]) {
     float* const turned = reinterpret_cast<float*>(patch);
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = threadIdx.x & 31, at = col + lane % 8;
     if (row >= p.M) return;
     const uint32_t rows = min(32u, p.M - row);
 #pragma unroll
-    for (int c = 0; c < NC; c += TURN) {
+    for (int j = 0; j < 8; ++j) turned[lane * 9 + j] = v[j];
+    __syncwarp();
+    if (at < p.N)
+        for (uint32_t r = lane / 8; r < rows; r += 4) out[uint64_t(row + r) * p.ldo + at] = from_f32<T>(turned[r * 9 + lane % 8]);
+    __syncwarp();
+}
+__device__ __forceinline__ void store_eight_as(void* out, int type, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[8]) {
+    if (type == ZC_BF16) store_eight(static_cast<__nv_bfloat16*>(out), p, row, col, patch, v);
+    else if (type == ZC_F16) store_eight(static_cast<__half*>(out), p, row, col, patch, v);
+    else store_eight(static_cast<float*>(out), p, row, col, patch, v);
+}
+// The same for NC columns of rows that start anywhere: 128 bytes of each row as 32 words, row by row out of shared memory (33 words a row), a word a
+// lane. A 16-bit row that starts between two words is shifted by half of one on the way; its first and its last value are stored alone. Eight
+// rows at a time and without branches: what bounds it is how long a warp waits for its own instructions (8192 x 8191 of BF16 over 1024 k: 58 us, sixteen
+// columns a round in FP32 98; aligned rows, by TMA, 37).
+template <typename T, int NC> __device__ __forceinline__ void store_turned(T* out, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    constexpr int PER = 4 / sizeof(T), CHUNK = 32 * PER;      // values of a word, columns of a round
+    uint32_t* const words = reinterpret_cast<uint32_t*>(patch);
+    const uint32_t lane = threadIdx.x & 31, rows = min(32u, p.M - row);
 #pragma unroll
-        for (int j = 0; j < TURN; ++j) turned[lane * PATCH + j] = v[c + j];
+    for (int c = 0; c < NC; c += CHUNK) {
+        if (col + c >= p.N) break;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            alignas(4) T w[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) w[k] = from_f32<T>(v[c + j * PER + k]);
+            words[lane * 33 + j] = *reinterpret_cast<const uint32_t*>(w);
+        }
         __syncwarp();
-        const uint32_t at = col + c + lane % TURN;
-        if (at < p.N)
-            for (uint32_t r = lane / TURN; r < rows; r += 32 / TURN) out[uint64_t(row + r) * p.ldo + at] = from_f32<T>(turned[r * PATCH + lane % TURN]);
+        const uint32_t limit = min(uint32_t(CHUNK), p.N - col - c);
+        T* to = out + uint64_t(row) * p.ldo + col + c;
+#pragma unroll 1
+        for (uint32_t r0 = 0; r0 < rows; r0 += 8) {
+            uint32_t w[8], next[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) w[i] = words[(r0 + i) * 33 + lane];
+            if constexpr (PER == 2) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) next[i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i, to += p.ldo) {
+                const uint32_t end = r0 + i < rows ? limit : 0;
+                if constexpr (PER == 1) {
+                    if (lane < end) *reinterpret_cast<uint32_t*>(to + lane) = w[i];
+                } else {
+                    uint16_t* const half = reinterpret_cast<uint16_t*>(to);
+                    const uint32_t odd = uint32_t(reinterpret_cast<uintptr_t>(to) >> 1) & 1, at = lane * 2 + odd;
+                    const uint32_t pair = odd ? __funnelshift_r(w[i], next[i], 16) : w[i];
+                    if (at + 1 < end) *reinterpret_cast<uint32_t*>(half + at) = pair;
+                    if (at + 1 == end) half[at] = uint16_t(pair);
+                    if (odd && lane == 0 && end) half[0] = uint16_t(w[i]);
+                }
+            }
+        }
         __syncwarp();
     }
 }
-template <int NC> __device__ __forceinline__ void store_turned_as(void* out, int type, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
-    if (type == ZC_BF16) store_turned(static_cast<__nv_bfloat16*>(out), p, row, col, patch, v);
-    else if (type == ZC_F16) store_turned(static_cast<__half*>(out), p, row, col, patch, v);
-    else store_turned(static_cast<float*>(out), p, row, col, patch, v);
-}
-// A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on; rows past `rows` and columns past `cols` are left out. Rows that
-// are 16-byte aligned leave by TMA: 128 (or 64) bytes of each through shared memory, swizzled so that neither side meets a bank twice.
+// A warp's 32 rows (one a lane) of NC columns, from (row, col) of the output on; rows and columns past the last one are left out. Rows that start and
+// end on 16 bytes leave by TMA: 128 (or 64) bytes of each through shared memory, swizzled so that neither side meets a bank twice.
 // Stored by the lanes, 16 bytes of a row each, they took 6,200 clocks a tile, and the waits of the copying and the issuing
-// thread queued behind them. Rows that are not aligned are turned (257 x 10007: 45 -> 23 us against values stored by the rows' own lanes).
-template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+// thread queued behind them. Others (only results of MX4 products can have such rows: ANY) are turned.
+template <bool ANY, typename T, int NC> __device__ __forceinline__ void store_rows(T* out, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
     const uint32_t lane = threadIdx.x & 31;
     if (row >= p.M) return;
-    if (p.aligned) {
+    if (!ANY || p.aligned) {
         constexpr int GROUP = NC * int(sizeof(T)) < 128 ? NC : 128 / int(sizeof(T)), CHUNK = 16 / sizeof(T), BYTES = GROUP * sizeof(T);
 #pragma unroll
         for (int c = 0; c < NC; c += GROUP) {
@@ -147,12 +189,12 @@ template <typename T, int NC> __device__ __forceinline__ void store_rows(T* out,
         }
         return;
     }
-    store_turned(out, p, row, col, patch, v);
+    if constexpr (ANY) store_turned(out, p, row, col, patch, v);
 }
-template <int NC> __device__ __forceinline__ void store_as(void* out, int type, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
-    if (type == ZC_BF16) store_rows(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
-    else if (type == ZC_F16) store_rows(static_cast<__half*>(out), map, p, row, col, patch, v);
-    else store_rows(static_cast<float*>(out), map, p, row, col, patch, v);
+template <bool ANY, int NC> __device__ __forceinline__ void store_as(void* out, int type, const CUtensorMap* map, const TilePlan& p, uint32_t row, uint32_t col, uint8_t* patch, const float (&v)[NC]) {
+    if (type == ZC_BF16) store_rows<ANY>(static_cast<__nv_bfloat16*>(out), map, p, row, col, patch, v);
+    else if (type == ZC_F16) store_rows<ANY>(static_cast<__half*>(out), map, p, row, col, patch, v);
+    else store_rows<ANY>(static_cast<float*>(out), map, p, row, col, patch, v);
 }
 // The quotient by the fast reciprocal (2 ulp): with the rounded division the epilogue of a gated tile took 26,000 clocks, more than the products
 // of 3,300 k. A denominator beyond 2^126 gives 0, which is silu's limit there.
@@ -168,8 +210,9 @@ constexpr uint32_t SM_SMEM = 228 * 1024, CTA_RESERVED = 1024, CTA_STATIC = 256, 
 constexpr uint32_t smem_share(uint32_t tmem_columns) { return tmem_columns * (SM_SMEM / 512) - CTA_RESERVED - CTA_STATIC; }
 
 template <bool MX4, bool GATED, int N> struct TileSmem {
+    static constexpr uint32_t patch = MX4 ? 5120 : 4096;      // a warp's, of the epilogue: 32 rows of 128 bytes (of 33 words where rows are turned), on 1024 bytes
     static constexpr uint32_t b = N / 2 * 128, block = A_BYTES + b + (MX4 ? (1 + N / 128) * 1024 : 0), depth = N == 256 ? 1 : 2, stage = depth * block;
-    static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, used = stages * stage + 8 * PATCH_BYTES + 1024;
+    static constexpr uint32_t stages = MX4 ? (N == 256 ? 5 : 3) : N == 256 ? 6 : 4, used = stages * stage + 8 * patch + 1024;
     static constexpr uint32_t bytes = smem_share(512);
     static constexpr bool shared = N == 128 || (MX4 && GATED);      // whether pairs may share a tile's K (the others are narrow where tiles are few)
     static_assert(used <= bytes && bytes <= CTA_SMEM_MAX, "shared memory of a tile CTA");
@@ -317,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     } else {
         constexpr int COLS = WIDTH / 2;                                 // output columns of a warp
         const uint32_t half = (warp - 2) >> 2, quarter = warp & 3;      // which columns; the 32 lanes of tensor memory a warp can read
-        uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * PATCH_BYTES;
+        uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * Smem::patch;
         uint32_t n = 0;
         for (uint32_t t = pair; t < p.tiles; t += pairs, ++n) {
             const Tile c = tile_at(p, t, WIDTH);
@@ -347,13 +390,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             }
             if constexpr (GATED) {
                 if (p.g) {
-                    store_as(p.g, p.saved_type, &maps.o[1], p, row, col, patch, v);
-                    store_as(p.u, p.saved_type, &maps.o[2], p, row, col, patch, w);
+                    store_as<MX4>(p.g, p.saved_type, &maps.o[1], p, row, col, patch, v);
+                    store_as<MX4>(p.u, p.saved_type, &maps.o[2], p, row, col, patch, w);
                 }
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = silu(v[i]) * w[i];
             }
-            store_as(c.z ? p.out[1] : p.out[0], p.out_type, &maps.o[c.z], p, row, col, patch, v);
+            store_as<MX4>(c.z ? p.out[1] : p.out[0], p.out_type, &maps.o[c.z], p, row, col, patch, v);
         }
         if (lane == 0) tma_store_done();
         __syncwarp();
@@ -364,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             cluster_sync();
             if (warp >= 2 && __all_sync(0xffffffffu, !*abort_flag)) {
                 const uint32_t quarter = warp & 3, share = WIDTH / p.splits;
-                uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * PATCH_BYTES;
+                uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * Smem::patch;
                 const Tile c = tile_at(p, pair, WIDTH);
                 const uint32_t row = c.m0 + rank * TILE_M + quarter * 32;
                 for (uint32_t j = part * share + ((warp - 2) >> 2) * 8; j < (part + 1) * share; j += 16) {
@@ -381,13 +424,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     }
                     if constexpr (GATED) {
                         if (p.g) {
-                            store_turned_as(p.g, p.saved_type, p, row, c.n0 + j, patch, v);
-                            store_turned_as(p.u, p.saved_type, p, row, c.n0 + j, patch, w);
+                            store_eight_as(p.g, p.saved_type, p, row, c.n0 + j, patch, v);
+                            store_eight_as(p.u, p.saved_type, p, row, c.n0 + j, patch, w);
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = silu(v[i]) * w[i];
                     }
-                    store_turned_as(c.z ? p.out[1] : p.out[0], p.out_type, p, row, c.n0 + j, patch, v);
+                    store_eight_as(c.z ? p.out[1] : p.out[0], p.out_type, p, row, c.n0 + j, patch, v);
                 }
             }
             __syncwarp();
