@@ -445,18 +445,23 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------------
 // Few tokens
 // ---------------------------------------------------------------------------------------------
-// D[M, tokens] = W . X^T: the weights are the 128 rows of a product, the tokens (at most 256, padded to a multiple of 16) its columns, so
-// a single token costs the tensor cores an eighth of what 128 would and the launch is what its bytes are: the weights, once. A CTA owns
-// one tile of 128 weight rows (of gate and of up) and one run of blocks of K; the CTAs of a cluster share a tile's K and add their partial
-// sums through distributed shared memory, in the order of their ranks. The lanes of the epilogue hold consecutive output columns of
-// a token, so plain stores are coalesced whatever the row stride.
+// D[M, tokens] = W . X^T: the weights are the 128 rows of a product, the tokens (64 at most, padded to a multiple of 16) its columns, so a single
+// token costs the tensor cores an eighth of what 128 would and the launch is what its bytes are: the weights, once. A CTA owns one tile of 128 weight
+// rows (of gate and of up) and one run of blocks of K; the CTAs of a cluster share a tile's K and add their partial sums through
+// distributed shared memory, in the order of their ranks. The lanes of the epilogue hold consecutive output columns of a token, so plain
+// stores are coalesced whatever the row stride.
 // A handful of plain tokens: every CTA quantises its own part of their K into shared memory (the epilogue warps, while the weights arrive),
-// in the swizzle TMA would have written (more are quantised by a launch of their own). The kernel before may still run while this one starts (programmatic launch): until it has
-// ended nothing is read but into L2, where a later write of it would arrive too.
-constexpr uint32_t FEW_THREADS = 192, FEW_STAGES = 8;
+// in the swizzle TMA would have written; more are quantised by a launch of their own.
+// The kernel before may still run while this one starts (programmatic launch): until it has ended nothing is read but into L2, where a later write
+// of it would arrive too.
+// What bounds it: one token, MX4 8192 x 4096, replayed back to back 6.4 us a call for 17.8 MB (2.7 us of HBM): 1.7 us until the first stage is there
+// (all CTAs ask for all weights at once: 10 TB/s out of L2), 1.3 for the products, 0.7 for the sums, 0.9 to leave the cluster, 1.5 until the next
+// kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 6.7.
+constexpr uint32_t FEW_THREADS = 192;
 // 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
 constexpr uint32_t FEW_TOKENS = 64;
-constexpr uint32_t FEW_SMEM = 110 * 1024;                                 // what a ring may take (two CTAs an SM)
+constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_STAGES = 6;                 // what a ring may take (two CTAs an SM), and its stages at most
+static_assert((FEW_SMEM - 1024) / (A_BYTES + 1024) <= FEW_STAGES, "stages of the smallest kind");
 // x is quantised inside where a CTA has at most so many rows of 256 of its columns (tokens x blocks; the four warps share them): MX4 2048 x 512, one block a
 // CTA, 1 / 4 / 8 / 12 / 16 tokens 3.4 / 3.6 / 4.3 / 4.8 / 5.3 us, by a launch of its own 4.6 / 4.8 / 4.8 / 5.0 / 5.2; 8192 x 4096, four blocks, 2 / 3 / 4
 // tokens 7.2 / 7.7 / 8.5 and 8.2 / 8.5 / 8.6.
@@ -599,19 +604,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     pdl_wait();
     pdl_launch_dependents();
 
-    const uint32_t b_bytes = fused ? 0 : p.n * 128, xtiles = p.n > 128 ? 2 : 1;      // token rows of a stage; scale tiles of the tokens
+    const uint32_t b_bytes = fused ? 0 : p.n * 128;      // token rows of a stage
     const uint32_t sf_off = MATS * A_BYTES + b_bytes;
     if (warp == 0) {
         if (elect_one()) {
             // slot, its round, segment and block are counted, not divided for: a division a stage is what the loop would wait for
             uint32_t it = 0, slot = 0, round = 0, seg = seg0, kb = kb0;
-            const bool two = xtiles == 2 && p.tokens > 128;
             bool ok = true;
             for (uint32_t k = k0; k < k1; ++k, ++it) {
                 const uint32_t a = ring + slot * p.stage;
                 if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
                 const uint32_t atoms = MX4 ? min(2u, p.ktiles - kb * 2) : 0;
-                mbar_expect(&full[slot], MATS * A_BYTES + b_bytes + atoms * 512 * (MATS + (fused ? 0 : two ? 2 : 1)));
+                mbar_expect(&full[slot], MATS * A_BYTES + b_bytes + atoms * 512 * (MATS + (fused ? 0 : 1)));
 #pragma unroll
                 for (uint32_t i = 0; i < MATS; ++i) {
                     if constexpr (A_MN) {
@@ -624,10 +628,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 }
                 if (!fused) {
                     tma_load_2d(a + MATS * A_BYTES, &maps.b[seg], &full[slot], kb * KB, 0);
-                    if constexpr (MX4) {
-                        bulk_load(a + sf_off + MATS * 1024, p.sfx + uint64_t(kb) * 1024, atoms * 512, &full[slot]);
-                        if (two) bulk_load(a + sf_off + MATS * 1024 + 1024, p.sfx + (uint64_t(p.ktiles) + kb * 2) * 512, atoms * 512, &full[slot]);
-                    }
+                    if constexpr (MX4) bulk_load(a + sf_off + MATS * 1024, p.sfx + uint64_t(kb) * 1024, atoms * 512, &full[slot]);
                 }
                 if (++slot == p.stages) { slot = 0; ++round; }
                 if (++kb == p.kblocks) { kb = 0; ++seg; }
@@ -660,8 +661,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                         if (j * 2 >= steps) break;
 #pragma unroll
                         for (uint32_t i = 0; i < MATS; ++i) tmem_copy_scales(sf + i * 8 + j * 4, dsa + i * 64 + j * 32);
-                        tmem_copy_scales(sf + MATS * 8 + j * 4 * xtiles, dsb + j * 32);
-                        if (xtiles == 2) tmem_copy_scales(sf + MATS * 8 + j * 8 + 4, dsb + 64 + j * 32);
+                        tmem_copy_scales(sf + MATS * 8 + j * 4, dsb + j * 32);
                     }
                 }
 #pragma unroll
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                         if constexpr (MX4) {
                             constexpr uint32_t odd = 2u << 29 | 2u << 4;
                             umma_mx4(tmem + i * p.n, da + i * (A_BYTES >> 4) + s * 2, db + s * 2, s & 1 ? p.idesc | odd : p.idesc, sf + i * 8 + (s >> 1) * 4,
-                                     sf + MATS * 8 + (s >> 1) * 4 * xtiles, more);
+                                     sf + MATS * 8 + (s >> 1) * 4, more);
                         } else {
                             umma_f16(tmem + i * p.n, da + i * (A_BYTES >> 4) + s * (A_MN ? 128 : 2), db + s * 2, p.idesc, more);
                         }
@@ -928,12 +928,11 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     if (splits > total) splits = total;
     p.kown = (total + splits - 1) / splits;
     p.splits = (total + p.kown - 1) / p.kown;
-    const uint32_t quantised = p.kown * (p.n * 128 + 1024), xtiles = p.n > 128 ? 2 : 1;
+    const uint32_t quantised = p.kown * (p.n * 128 + 1024);
     const bool fused = plain && p.tokens * p.kown <= FEW_PLAIN_ROWS;
-    p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? xtiles * 1024 : 0));
+    p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? 1024 : 0));
     const uint32_t room = FEW_SMEM - 1024 - (fused ? quantised : 0);
     p.stages = room / p.stage;
-    if (p.stages > FEW_STAGES) p.stages = FEW_STAGES;
     if (p.stages > p.kown) p.stages = p.kown;
     uint32_t bytes = p.stages * p.stage;
     const uint32_t sums = p.splits > 1 ? mats * p.tokens * 512 : 0;
@@ -941,7 +940,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.resident = fused ? (bytes > sums ? bytes : (sums + 1023) / 1024 * 1024) : 0;
     p.smem = 1024 + (fused ? p.resident + quantised : bytes);
     p.sf_column = mats * p.n;
-    p.sf_columns = mx4 ? mats * 8 + 8 * xtiles : 0;
+    p.sf_columns = mx4 ? mats * 8 + 8 : 0;
     p.tmem_columns = 32;
     while (p.tmem_columns < p.sf_column + p.stages * p.sf_columns) p.tmem_columns *= 2;
     if (p.smem < smem_share(p.tmem_columns)) p.smem = smem_share(p.tmem_columns);
@@ -957,7 +956,6 @@ template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, Fe
     if (rc != ZC_OK) return rc;
     return launched(launch_after(kernel, dim3((p.M + TILE_M - 1) / TILE_M * p.splits), FEW_THREADS, p.smem, p.splits, s, maps, p), "dense product of few tokens");
 }
-
 
 struct Mx4Arg { const void *codes, *scales; };
 

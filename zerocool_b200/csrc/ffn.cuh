@@ -46,18 +46,22 @@ template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __
 template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32(float v) { return v; }
 
-// Eight consecutive values of a row. VEC: the row is 16-byte aligned.
+// Eight consecutive values of a row. VEC: the row is 16-byte aligned. Not through the read-only path: a kernel of these starts while the kernel
+// before it still writes (programmatic launch), and that path may keep what it read before.
 template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    alignas(16) T raw[8];
     if constexpr (VEC) {
-        T raw[8];
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) * 8 / 16; ++i) reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
+        for (uint32_t i = 0; i < sizeof(T) * 8 / 16; ++i) reinterpret_cast<uint4*>(raw)[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) reinterpret_cast<float*>(raw)[i] = __ldca(reinterpret_cast<const float*>(p) + i);
+            else reinterpret_cast<unsigned short*>(raw)[i] = __ldca(reinterpret_cast<const unsigned short*>(p) + i);
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
 }
 #endif
 

@@ -14,7 +14,7 @@ constexpr int FLIGHT = 4;                       // rows of a warp, all of their 
 // A CTA takes 32 rows x 256 columns, whose scales are every fourth 32-bit word of two tiles (gathered in shared memory; words of rows and
 // columns past the last one are written 0, so the grid covers whole tiles). Four lanes share a block of 32: lane l holds columns 8 l .. 8 l + 7 of
 // the 256, a warp its four rows at once.
-template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t cols, uint64_t ld,
+template <typename T, bool VEC> __global__ void __launch_bounds__(256) quantize_kernel(const T* x, uint32_t rows, uint32_t cols, uint64_t ld,
                                                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ uint32_t words[2][QT_ROWS];
     const uint32_t row0 = blockIdx.x * QT_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * QT_COLS + lane * 8;
@@ -56,8 +56,8 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) dequantiz
 #pragma unroll
     for (int i = 0; i < FLIGHT; ++i) {
         const uint32_t r = min(r0 + i, rows - 1);
-        word[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + uint64_t(r) * (cols >> 1) + (col >> 1)));
-        s[i] = __ldg(scales + mx4_scale_at(r, col / 32, (cols + 127) / 128));
+        word[i] = __ldcg(reinterpret_cast<const uint32_t*>(codes + uint64_t(r) * (cols >> 1) + (col >> 1)));
+        s[i] = __ldca(scales + mx4_scale_at(r, col / 32, (cols + 127) / 128));
     }
 #pragma unroll
     for (int i = 0; i < FLIGHT; ++i) {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restr
     pdl_wait();
     pdl_launch_dependents();
     for (uint32_t j = 0; j < 4; ++j)
-        if (row < rows && b0 + j < blocks) word |= uint32_t(from[uint64_t(row) * blocks + b0 + j]) << (8 * j);
+        if (row < rows && b0 + j < blocks) word |= uint32_t(__ldca(from + uint64_t(row) * blocks + b0 + j)) << (8 * j);
     *reinterpret_cast<uint32_t*>(to + (uint64_t(blockIdx.x) * gridDim.y + blockIdx.y) * 512 + (threadIdx.x & 31) * 16 + (threadIdx.x >> 5) * 4) = word;
 }
 
