@@ -437,7 +437,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync();
+    if (Smem::shared && p.splits > 1) cluster_leave();       // (the arrivals at the leader's barriers came before the sums)
+    else cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
@@ -454,9 +455,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // in the swizzle TMA would have written; more are quantised by a launch of their own.
 // The kernel before may still run while this one starts (programmatic launch): until it has ended nothing is read but into L2, where a later write
 // of it would arrive too.
-// What bounds it: one token, MX4 8192 x 4096, replayed back to back 6.4 us a call for 17.8 MB (2.7 us of HBM): 1.7 us until the first stage is there
-// (all CTAs ask for all weights at once: 10 TB/s out of L2), 1.3 for the products, 0.7 for the sums, 0.9 to leave the cluster, 1.5 until the next
-// kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 6.7.
+// What bounds it: one token, MX4 8192 x 4096, replayed back to back 6.1 us a call for 17.8 MB (2.7 us of HBM): 1.7 us until the first stage is there
+// (all CTAs ask for all weights at once: 10 TB/s out of L2), 1.3 for the products, 0.7 for the sums, 0.6 to leave the cluster, 1.5 until the next
+// kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 0.2 us more.
 constexpr uint32_t FEW_THREADS = 192;
 // 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
 constexpr uint32_t FEW_TOKENS = 64;
@@ -721,8 +722,12 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
             __syncwarp();
         }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (p.splits > 1) cluster_sync();
+    else __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
     if (p.splits > 1) {
-        cluster_sync();
         if (warp >= 2 && !*abort_flag) {
             const uint32_t row = lane * 4;           // four rows a lane, a token a warp
             for (uint32_t t = rank + (warp - 2) * p.splits; t < p.tokens; t += 4 * p.splits) {
@@ -742,12 +747,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
             }
         }
         __syncwarp();
-        cluster_sync();          // no CTA leaves while another may still read its sums
+        cluster_leave();         // no CTA leaves while another may still read its sums
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
 }
 
 // dg = dh u s (1 + g (1 - s)), du = dh g s, in FP32; rounded to the operands' type, as the tensor cores take them (the gradients' error is that

@@ -122,6 +122,11 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {      
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
     return there;
 }
+// The same for CTAs that have only loaded from one another (and hold what they loaded): nothing is handed over, so no earlier store is waited for.
+__device__ __forceinline__ void cluster_leave() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_index() { uint32_t r; asm("mov.u32 %0, %%clusterid.x;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_count() { uint32_t r; asm("mov.u32 %0, %%nclusterid.x;" : "=r"(r)); return r; }
