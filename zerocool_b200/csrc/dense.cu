@@ -461,8 +461,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 constexpr uint32_t FEW_THREADS = 192;
 // 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
 constexpr uint32_t FEW_TOKENS = 64;
-// What a ring may take where SMs have two CTAs (one alone takes what there is: 16-bit block of 16384 x 4096, 64 tokens, two stages 65 us, five 52), and
-// its stages at most.
+// What a ring may take where SMs have two CTAs, and its stages at most. A CTA that has its SM alone takes what there is (16-bit block of 16384 x 4096,
+// 64 tokens: two stages 65 us, five 52), unless it is one of a cluster: sixteen clusters of eight such do not all fit (2048 x 2048: 9.9 us, 6.5).
 constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_STAGES = 6;
 // x is quantised inside where a CTA has at most so many rows of 256 of its columns (tokens x blocks; the four warps share them): MX4 2048 x 512, one block a
 // CTA, 1 / 4 / 8 / 12 / 16 tokens 3.4 / 3.6 / 4.3 / 4.8 / 5.3 us, by a launch of its own 4.6 / 4.8 / 4.8 / 5.0 / 5.2; 8192 x 4096, four blocks, 2 / 3 / 4
@@ -933,7 +933,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     const uint32_t quantised = p.kown * (p.n * 128 + 1024);
     const bool fused = plain && p.tokens * p.kown <= FEW_PLAIN_ROWS;
     p.stage = mats * (A_BYTES + (mx4 ? 1024 : 0)) + (fused ? 0 : p.n * 128 + (mx4 ? 1024 : 0));
-    const uint32_t room = (mtiles * p.splits <= sms ? CTA_SMEM_MAX : FEW_SMEM) - 1024 - (fused ? quantised : 0);
+    const uint32_t room = (p.splits == 1 && mtiles <= sms ? CTA_SMEM_MAX : FEW_SMEM) - 1024 - (fused ? quantised : 0);
     p.stages = room / p.stage;
     if (p.stages > FEW_STAGES) p.stages = FEW_STAGES;
     if (p.stages > p.kown) p.stages = p.kown;
