@@ -128,7 +128,7 @@ SIZES = [(1, 1, 32), (2, 128, 64), (7, 129, 96), (16, 64, 128), (17, 300, 160), 
          (255, 33, 2048), (257, 513, 320), (300, 1000, 992),
          (1, 260, 4128), (5, 300, 8192), (33, 200, 8224), (128, 140, 2080), (3, 20000, 96), (31, 2400, 1056),
          (1300, 2600, 160), (700, 4100, 416), (129, 9000, 2080),
-         (200, 300, 8224), (260, 141, 3104), (1000, 520, 6400), (129, 1, 32), (300, 7, 96), (1, 7, 32), (64, 64, 64), (65, 64, 64), (400, 600, 4000), (1000, 520, 9312)]
+         (200, 300, 8224), (260, 141, 3104), (1000, 520, 6400), (129, 1, 32), (300, 7, 96), (1, 7, 32), (64, 64, 64), (65, 64, 64), (400, 600, 4000), (1000, 520, 9312), (40, 300, 512), (40, 300, 544), (60, 300, 2048), (50, 300, 2080)]
 
 
 @pytest.mark.parametrize("tokens,rows,cols", SIZES)
@@ -239,7 +239,7 @@ def test_no_tokens(ffn):
 
 BLOCKS = [(1, 8, 8), (1, 64, 128), (5, 72, 136), (16, 128, 64), (33, 64, 200), (127, 136, 128), (128, 64, 256), (129, 264, 72), (200, 520, 392), (256, 128, 512), (513, 320, 264),
           (1, 2056, 1160), (9, 4096, 136), (65, 520, 4104), (128, 1032, 1032), (2, 40, 20008), (1100, 264, 2600), (1500, 2056, 136),
-          (200, 2056, 136), (130, 40, 4104), (1500, 136, 136), (900, 1032, 520), (130, 8, 8), (300, 16, 8), (64, 8, 264), (70, 264, 8), (900, 2312, 520), (900, 520, 1200), (2400, 520, 520)]
+          (200, 2056, 136), (130, 40, 4104), (1500, 136, 136), (900, 1032, 520), (130, 8, 8), (300, 16, 8), (64, 8, 264), (70, 264, 8), (900, 2312, 520), (900, 520, 1200), (2400, 520, 520), (40, 512, 136), (40, 520, 264), (60, 2048, 72), (50, 2056, 1032)]
 
 
 @pytest.mark.parametrize("tokens,hidden,width", BLOCKS)

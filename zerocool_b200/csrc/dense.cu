@@ -459,8 +459,15 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // (all CTAs ask for all weights at once: 10 TB/s out of L2), 1.3 for the products, 0.7 for the sums, 0.6 to leave the cluster, 1.5 until the next
 // kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 0.2 us more.
 constexpr uint32_t FEW_THREADS = 192;
-// 16-bit gate and up of 8192 x 4096: 64 tokens 31 us here and 42 in tiles of pairs, 128 tokens 57 and 42; MX4 8192 x 4096: 12 and 12, 18 and 15.
+// Which calls: up to 64 tokens, unless K is short, where the tokens' sums over the cluster cost more than the weights. Rows x K, here / in tiles of pairs, us,
+// of MX4 product | MX4 block | 16-bit block. 2048 x 512: 25 tokens 4.1 / 4.1 | 7.5 / 7.6 | 7.2 / 7.2, 32 tokens 4.6 / 4.1 | 7.6 / 7.6 | 7.5 / 7.2, 33 tokens
+// 4.9 / 4.1 | 8.2 / 8.2 | 8.2 / 7.2, 64 tokens 6.2 / 4.4 | 10.4 / 8.2 | 9.3 / 7.2. 1024 x 1024: 48 tokens 4.6 / 4.6 | 8.2 / 8.9 | 8.3 / 8.2, 64 tokens
+// 5.3 / 4.6 | 8.9 / 8.3 | 8.3 / 8.2. 2048 x 2048: 33 tokens 5.7 / 5.4 | 8.9 / 9.6 | 9.7 / 10.3, 64 tokens 6.7 / 5.7 | 10.5 / 9.7 | 12.2 / 10.6. 1024 x 4096,
+// 64 tokens: 5.7 / 6.7 | 9.6 / 12.3 | 11.3 / 12.4. 8192 x 8192, 64 tokens: 12.5 / 14.1 | 21.9 / 22.4 | 49 / 55. What the rule gives away: few rows of K = 2048
+// (512 x 2048, 49 tokens 4.6 / 5.2 | 8.2 / 9.6 | 8.3 / 9.3; 64 tokens 5.2 / 5.2 | 8.9 / 9.6 | 9.3 / 9.3). 128 tokens of 8192 x 4096: MX4 18 / 15, 16-bit
+// block 57 / 42. dx, whose K is two segments, stays here up to 64 tokens (hidden x ffn, 2048 x 1024 8.8 / 10.3, 4096 x 4096 19 / 24, 2048 x 512 8.2 / 8.2).
 constexpr uint32_t FEW_TOKENS = 64;
+bool takes_few(uint32_t tokens, uint32_t k) { return tokens <= 32 || (tokens <= 48 && k > 512) || (tokens <= FEW_TOKENS && k > 2048); }
 // What a ring may take where SMs have two CTAs, and its stages at most. A CTA that has its SM alone takes what there is (16-bit block of 16384 x 4096,
 // 64 tokens: two stages 65 us, five 52), unless it is one of a cluster: sixteen clusters of eight such do not all fit (2048 x 2048: 9.9 us, 6.5).
 constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_STAGES = 6;
@@ -918,7 +925,7 @@ template <typename Plan> void set_k(Plan& p, uint32_t k, uint32_t block, uint32_
 }
 void set_tile_k(TilePlan& p, uint32_t k, uint32_t block, bool narrow) { narrow ? set_k(p, k, 2 * block, 8) : set_k(p, k, block); }
 
-// Cuts a call of few tokens (at most FEW_TOKENS). kblocks, ksteps, segs, M, tokens, cols are set; plain: x is to be quantised.
+// Cuts a call of few tokens. kblocks, ksteps, segs, M, tokens, cols are set; plain: x is to be quantised.
 void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.n = (p.tokens + 15) / 16 * 16;
     const uint32_t total = p.kblocks * p.segs, mtiles = (p.M + TILE_M - 1) / TILE_M;
@@ -982,7 +989,7 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     Device d;
     if ((rc = current_device(d)) != ZC_OK) return rc;
     TileMaps maps{};
-    if (tokens <= FEW_TOKENS) {
+    if (takes_few(tokens, cols)) {
         FewPlan p{};
         p.M = rows; p.tokens = tokens; p.segs = 1;
         set_k(p, cols, 256);
@@ -1070,7 +1077,7 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
     if ((rc = current_device(d)) != ZC_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     TileMaps maps{};
-    if (tokens <= FEW_TOKENS) {
+    if (takes_few(tokens, hidden)) {
         FewPlan p{};
         p.M = ffn; p.tokens = tokens; p.segs = 1;
         set_k(p, hidden, 64);
