@@ -120,3 +120,15 @@ def test_reference_gradient_against_differences():
             args = [v + step if v is t else v for v in (x, gate, up)]
             back = [v - step if v is t else v for v in (x, gate, up)]
             assert abs((loss(*args) - loss(*back)).item() / 2e-6 - want.reshape(-1)[i].item()) < 1e-6 * (1 + want.abs().max().item())
+
+
+@pytest.mark.parametrize("wrong", [None, 3, torch.zeros(()), torch.zeros(4)])
+def test_arguments_of_the_wrong_kind_are_value_errors(wrong):
+    from zerocool_b200 import ffn
+    x = torch.zeros(2, 32, dtype=torch.bfloat16)
+    for call in (lambda: ffn.mx4_dequantize(wrong), lambda: ffn.Mx4(wrong, torch.zeros(512, dtype=torch.uint8)),
+                 lambda: ffn.Mx4(torch.zeros(1, 16, dtype=torch.uint8), wrong), lambda: ffn.mx4_from_rows(wrong, torch.zeros(1, 1, dtype=torch.uint8)),
+                 lambda: ffn.mx4_from_rows(torch.zeros(1, 16, dtype=torch.uint8), wrong), lambda: ffn.mx4_quantize(x, out=3),
+                 lambda: ffn.gated_forward(x, wrong, x), lambda: ffn.gated_backward(x, x, wrong, x, x, x)):
+        with pytest.raises(ValueError):
+            call()

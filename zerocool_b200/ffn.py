@@ -82,6 +82,16 @@ def _whole(name, t, shape, dtype, device):
         _same_device(device, **{name: t})
 
 
+def _tensor(name, t):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix")
+
+
+def _mx4(name, q):
+    if not isinstance(q, Mx4):
+        raise ValueError(f"{name} must be an Mx4 (mx4_quantize)")
+
+
 def _same_device(device, **others):
     for name, t in others.items():
         if t is not None and t.device != device:
@@ -119,7 +129,10 @@ class Mx4:
     tile layout of include/zc_ffn.h. Holds the tensors; copies nothing."""
 
     def __init__(self, codes, scales):
-        if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
+        _tensor("codes", codes)
+        if not isinstance(scales, torch.Tensor):
+            raise ValueError("scales must be a tensor")
+        if codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
             raise ValueError("codes must be contiguous uint8 [rows, cols / 2], cols a multiple of 32")
         if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.device != codes.device or \
                 scales.numel() != _scale_bytes(codes.shape[0], codes.shape[1] * 2):
@@ -157,6 +170,7 @@ def mx4_quantize(x, out=None):
     if out is None:
         out = Mx4.empty(rows, cols, x.device)
     else:
+        _mx4("out", out)
         if (out.rows, out.cols) != (rows, cols):
             raise ValueError(f"out must be [{rows}, {cols}]")
         _same_device(x.device, out=out)
@@ -166,7 +180,8 @@ def mx4_quantize(x, out=None):
 
 def mx4_dequantize(q, dtype=None, out=None):
     """The values of an Mx4 (default bfloat16, which holds each of them exactly)."""
-    dtype = out.dtype if dtype is None and out is not None else dtype or torch.bfloat16
+    _mx4("q", q)
+    dtype = getattr(out, "dtype", None) if dtype is None and out is not None else dtype or torch.bfloat16
     code = _code(dtype)
     out, ld = _out(out, q.rows, q.cols, dtype, q.device)
     _call(q.device, "zc_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, out.data_ptr(), code, ld)
@@ -175,7 +190,9 @@ def mx4_dequantize(q, dtype=None, out=None):
 
 def mx4_from_rows(codes, scales):
     """A checkpoint's codes [rows, cols / 2] and row-major scales [rows, cols / 32] (both uint8) -> Mx4 (the codes are not copied)."""
-    if codes.dim() != 2 or codes.dtype != torch.uint8:
+    _tensor("codes", codes)
+    _tensor("scales", scales)
+    if codes.dtype != torch.uint8:
         raise ValueError("codes must be uint8 [rows, cols / 2]")
     if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], codes.shape[1] // 16):
         raise ValueError("scales must be contiguous uint8 [rows, cols / 32]")
@@ -206,7 +223,7 @@ def _mx4_product(entry, x, weights, out_dtype, out):
     if xcols != cols:
         raise ValueError(f"x has {xcols} columns, the weights {cols}")
     _same_device(device, x=x, weights=weights[-1])
-    out_dtype = out.dtype if out_dtype is None and out is not None else out_dtype or torch.bfloat16
+    out_dtype = getattr(out, "dtype", None) if out_dtype is None and out is not None else out_dtype or torch.bfloat16
     code = _code(out_dtype)
     out, out_ld = _out(out, tokens, rows, out_dtype, device)
     pointers = [p for m in weights for p in (m.codes.data_ptr(), m.scales.data_ptr())]
@@ -230,6 +247,7 @@ def gated_forward(x, gate, up, save=False, save_dtype=torch.float32, out=None):
     two more roundings in the gradients."""
     code = _code(getattr(x, "dtype", None), sixteen=True)
     ld = _matrix("x", x)
+    _tensor("gate", gate)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
     dtype, device = x.dtype, x.device
     _whole("gate", gate, (ffn, hidden), dtype, device)
@@ -252,6 +270,7 @@ def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
     """The gradient of gated_forward -> (dx, dgate, dup) in the operands' dtype (None for what is not asked for)."""
     code = _code(getattr(x, "dtype", None), sixteen=True)
     x_ld = _matrix("x", x)
+    _tensor("gate", gate)
     (tokens, hidden), ffn = x.shape, gate.shape[0]
     dtype, device = x.dtype, x.device
     _whole("gate", gate, (ffn, hidden), dtype, device)
