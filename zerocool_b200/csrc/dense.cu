@@ -197,8 +197,14 @@ template <bool ANY, int NC> __device__ __forceinline__ void store_as(void* out, 
     else store_rows<ANY>(static_cast<float*>(out), map, p, row, col, patch, v);
 }
 // The quotient by the fast reciprocal (2 ulp): with the rounded division the epilogue of a gated tile took 26,000 clocks, more than the products
-// of 3,300 k. A denominator beyond 2^126 gives 0, which is silu's limit there.
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
+// of 3,300 k. It gives 0 for a denominator beyond 2^126, so far below zero, where 1 + e^-v is e^-v to the last bit, silu(v) = v e^v, its exponential in two
+// factors: neither of them leaves FP32's normal range before the result does.
+constexpr float FAR_GATE = -64.0f;
+__device__ __forceinline__ float silu(float v) {
+    const bool far = v < FAR_GATE;
+    const float t = expf(far ? 0.5f * v : -v);
+    return far ? v * t * t : __fdividef(v, 1.0f + t);
+}
 
 // A stage is `depth` blocks of K, loaded and released together: with 128 columns a block is worth 256 clocks of products, and waiting for it,
 // releasing it and going round cost the issuing thread 300 beside its products' 40 each.
