@@ -1,5 +1,7 @@
 """Dense feed-forward operators on the GPU where their arithmetic, their plans and their arguments end (definitions: tests/mx4_reference.py;
 the tolerances are those of tests/test_ffn_gpu.py, and what a test adds to them stands beside it)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -29,3 +31,38 @@ def test_far_gates_keep_their_values(ffn, tokens):
     h, g, u = ffn.gated_forward(x, gate, up, save=True)
     want = ref.silu(g.double()) * u.double()
     close(h, want, 2.0 ** -20 * want.abs() + 2.0 ** -150 * u.double().abs())
+
+
+def gradient(ffn, dh, x, gate, up, g, u, want_x=True, want_w=True):
+    """zc_gated_backward with dg and du in the test's own hands -> dg, du, dx, dgate, dup."""
+    (tokens, width), hidden, new = dh.shape, x.shape[1], x.new_empty
+    dg, du = new((tokens, width)), new((tokens, width))
+    dx, dgate, dup = new((tokens, hidden)) if want_x else None, new((width, hidden)) if want_w else None, new((width, hidden)) if want_w else None
+    at = lambda t: ctypes.c_void_p(None if t is None else t.data_ptr())  # noqa: E731
+    rc = ffn.load_library().zc_gated_backward(at(dh), dh.stride(0), at(x), x.stride(0), at(gate), at(up), at(g), at(u), ffn.CODES[g.dtype], ffn.CODES[x.dtype], tokens, hidden, width,
+                                              at(dg), at(du), at(dx), at(dgate), at(dup), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, ffn.load_library().zc_last_error()
+    return dg, du, dx, dgate, dup
+
+
+def elementwise_slack(dh, g, u):
+    """dg and du are computed in FP32: 2^-18 of the terms before they cancel in 1 + g (1 - s) (fast exponential and reciprocal; the exponential's
+    error grows with its argument, 2 + |1.18 g| units of 2^-23), and a sigmoid, or a product on the way to it, that may be subnormal."""
+    s, each = torch.sigmoid(g), 2.0 ** -18 + (2 + 1.18 * g.abs()) * 2.0 ** -23
+    under = 2.0 ** -149 * (1 + g.abs())
+    return each * (dh * u * s).abs() * (1 + g.abs() * (1 - s)) + under, each * (dh * g * s).abs() + under
+
+
+@pytest.mark.parametrize("saved", [torch.float32, torch.bfloat16])
+def test_far_gates_keep_their_gradients(ffn, saved):
+    """Gates of -60 to -160 whose dh and u are large enough for a gradient that is far above the smallest number."""
+    g = -torch.linspace(60, 160, 64, device="cuda").repeat(3, 1).to(saved)
+    u = torch.full_like(g, 2.0 ** 60)
+    dh = torch.full((3, 64), 2.0 ** 40, dtype=torch.bfloat16, device="cuda")
+    x, gate, up = (torch.zeros(r, 8, dtype=torch.bfloat16, device="cuda") for r in (3, 64, 64))
+    dg, du, *_ = gradient(ffn, dh, x, gate, up, g, u)
+    d = [t.double() for t in (dh, g, u)]
+    want = ref.gated_gradient(d[0], x.double(), gate.double(), up.double(), d[1], d[2])[:2]
+    for got, right, slack in zip((dg, du), want, elementwise_slack(*d)):
+        close(got, right, slack)
+    assert bool((dg[:, :40] < 0).all()) and bool((du[:, :40] < 0).all())
