@@ -10,7 +10,8 @@
  *    which loads its kernels). Calls on different streams share nothing.
  *  - Zero tokens (rows) is a valid call: nothing is read or written, but that gradients of the weights become zero.
  *  - Results do not depend on what else runs and are the same bits on every call: no atomics, a fixed order of sums.
- *  - A wait inside a kernel is bounded; one that runs out raises ZC_STATUS_TIMEOUT in a word of the device (zc_ffn_status).
+ *  - A wait inside a kernel is bounded (zc_ffn_wait_limit); one that runs out raises ZC_STATUS_TIMEOUT in a word of the device (zc_ffn_status).
+ *    The results of that call are not meaningful then; the kernel ends what it has started and the device stays usable.
  *
  * Microscaled matrix (MX4) of [rows, cols], cols a multiple of 32: the MXFP4 format of the OCP Microscaling Formats specification v1.0.
  *  - codes: [rows, cols / 2] bytes, two e2m1 values a byte (sign, two exponent bits, one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6),
@@ -77,6 +78,11 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
 
 /* Waits for `stream` and returns the current device's status word of these operators (then clears it). */
 int zc_ffn_status(void* stream, uint32_t* status);
+
+/* How often a wait inside the products' kernels polls before it gives up, for the calls of this process that follow (a captured call keeps what it was
+ * captured with): a poll takes about a microsecond at most. before (may be NULL) receives the limit so far. */
+#define ZC_FFN_WAIT_POLLS 1048576u   /* the limit that holds until the first such call */
+int zc_ffn_wait_limit(uint32_t polls, uint32_t* before);
 
 #ifdef __cplusplus
 }

@@ -66,3 +66,57 @@ def test_far_gates_keep_their_gradients(ffn, saved):
     for got, right, slack in zip((dg, du), want, elementwise_slack(*d)):
         close(got, right, slack)
     assert bool((dg[:, :40] < 0).all()) and bool((du[:, :40] < 0).all())
+
+
+# -- waits that run out --------------------------------------------------------------------------------------------------------
+
+@pytest.fixture
+def short_waits(ffn):
+    """A limit of the kernels' waits that a test makes run out: they give up, drain what they have started and return."""
+    yield ffn.wait_limit
+    ffn.wait_limit()
+    torch.cuda.synchronize()
+    ffn.status()
+
+
+def every_plan(ffn):
+    """Calls of every kernel: few tokens alone and in clusters, quantised inside or not, with ring wraps; tiles of either width, alone, many a pair, K shared."""
+    x16 = {(t, k): randn((t, k), 1, dtype=torch.bfloat16) for t, k in ((1, 4128), (19, 2080), (60, 2048), (200, 8224), (300, 992), (700, 4104), (129, 2056))}
+    w4 = {(n, k): ffn.mx4_quantize(randn((n, k), 2, 0.1)) for n, k in ((300, 4128), (14300, 2080), (300, 8224), (1000, 992), (9000, 992))}
+    w16 = {(n, k): randn((n, k), 3, 0.1, torch.bfloat16) for n, k in ((520, 4104), (136, 2056), (2600, 2056), (520, 2048), (4104, 992))}
+    calls = [lambda: ffn.mx4_linear(x16[1, 4128], w4[300, 4128]), lambda: ffn.mx4_gated(x16[19, 2080], w4[14300, 2080], w4[14300, 2080]),
+             lambda: ffn.mx4_linear(x16[19, 2080], w4[14300, 2080]), lambda: ffn.mx4_linear(x16[200, 8224], w4[300, 8224]), lambda: ffn.mx4_gated(x16[200, 8224], w4[300, 8224], w4[300, 8224]),
+             lambda: ffn.mx4_linear(x16[300, 992], w4[1000, 992]), lambda: ffn.mx4_linear(x16[300, 992], w4[9000, 992]), lambda: ffn.mx4_gated(x16[300, 992], w4[9000, 992], w4[9000, 992])]
+    for (t, k), (n, _) in (((60, 2048), (520, 2048)), ((700, 4104), (520, 4104)), ((129, 2056), (136, 2056)), ((129, 2056), (2600, 2056)), ((300, 992), (4104, 992))):
+        g, u, dh = (randn((t, n), s) for s in (4, 5, 6))
+        calls.append(lambda x=x16[t, k], w=w16[n, k]: ffn.gated_forward(x, w, w))
+        calls.append(lambda x=x16[t, k], w=w16[n, k], g=g, u=u, dh=dh.bfloat16(): torch.cat([v.reshape(-1) for v in ffn.gated_backward(dh, x, w, w, g, u)]))
+    return calls
+
+
+def test_waits_that_run_out_are_reported_and_leave_the_device_usable(ffn, short_waits):
+    """No wait is granted a poll: every product gives up with its copies in flight, says so, and the next call is right."""
+    calls = every_plan(ffn)
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    assert ffn.status() == 0
+    for i, call in enumerate(calls):
+        assert short_waits(0) == ffn.WAIT_POLLS
+        call()
+        assert ffn.status() == 2 and ffn.status() == 0, i       # ZC_STATUS_TIMEOUT, taken by the call that returns it
+        assert short_waits() == 0
+        assert torch.equal(call(), want[i]) and ffn.status() == 0, i
+
+
+@pytest.mark.parametrize("polls", [1, 2, 3, 4, 6, 8, 12, 20])
+def test_waits_that_run_out_somewhere(ffn, short_waits, polls):
+    """Limits at which some waits run out and others do not: a call says that it gave up, or its result is right."""
+    for i, call in enumerate(every_plan(ffn)):
+        want = call()
+        for _ in range(3):
+            short_waits(polls)
+            got = call()
+            gave_up = ffn.status()
+            short_waits()
+            assert gave_up in (0, 2) and (gave_up or torch.equal(got, want)), i
+        assert torch.equal(call(), want) and ffn.status() == 0, i

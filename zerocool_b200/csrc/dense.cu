@@ -14,8 +14,10 @@
 // the 48 KB of a single CTA's widest tile, whose loop L2 bounded (11 TB/s: 150 us for MX4 8192 x 8192 x 4096).
 // Two accumulators where they fit, so that the drain is hidden. MX4 products keep their scales in tensor memory too (32 columns a stage),
 // which leaves one of 256: the next tile waits until it is in registers, not until it is stored.
-// Every wait is bounded (POLL_LIMIT): one that runs out raises ZC_STATUS_TIMEOUT and the CTA's abort flag; its roles leave their
-// loops, wait for the copies and products in flight, and the tensor memory is freed.
+// Every wait is bounded (POLL_LIMIT polls, unless zc_ffn_wait_limit says otherwise): one that runs out raises ZC_STATUS_TIMEOUT and the abort
+// flag, of both CTAs of a pair and all pairs of a tile; the roles leave their loops, and no CTA frees its tensor memory or ends before the
+// copies and products that it has started have ended. A copy has ended when its stage is released; the copying thread therefore waits for the
+// last stages too (while the others drain the last tile), and where that is cut short, for the bytes themselves.
 #include "ffn.cuh"
 #include "tcgen05.cuh"
 #include <atomic>
@@ -48,6 +50,8 @@ int check_matrix(const char* who, const void* p, int dtype, uint32_t rows, uint3
 namespace {
 
 __device__ uint32_t ffn_status_word;     // the device's status word of these operators (zc_ffn_status)
+static_assert(POLL_LIMIT == ZC_FFN_WAIT_POLLS, "the limit that zc_ffn.h states");
+std::atomic<uint32_t> wait_polls{POLL_LIMIT};      // of the launches that follow (zc_ffn_wait_limit)
 
 constexpr uint32_t TILE_M = 128, THREADS = 320;           // rows of a CTA
 constexpr uint32_t A_BYTES = TILE_M * 128;
@@ -75,6 +79,7 @@ struct TilePlan {
     Divisor band, last;                 // tiles of a band of eight row tiles; row tiles of the last, shorter band
     uint32_t splits, kown;              // pairs that share a tile's K (then a cluster has one tile), stages of each
     uint32_t idesc;
+    uint32_t polls;                     // of a wait
     uint32_t ktiles;                    // MX4: scale tiles along K
     void* out[2];
     uint64_t ldo;
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;       // (CTA_STATIC bytes at most)
-    __shared__ uint32_t tmem_s, abort_s;
+    __shared__ uint32_t tmem_s, abort_s, issued_s;       // issued_s: the stages that this CTA's copying thread has started
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank() & 1, part = cluster_rank() >> 1, lead = part * 2;            // lead: the leader's rank in the cluster
     const uint32_t pair = cluster_index(), pairs = cluster_count();
@@ -240,6 +245,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     const uint32_t seg0 = k0 >= p.kblocks, kb0 = k0 - (seg0 ? p.kblocks : 0);                         // (at most two segments)
     uint32_t* const status = &ffn_status_word;
     volatile uint32_t* const abort_flag = &abort_s;
+    const auto give_up = [&] {      // by one thread of a role whose wait ran out: no other CTA of the cluster waits for its limit as well
+        for (uint32_t r = 0; r < 2 * p.splits; ++r) store_cluster_word(map_to(smem_addr(&abort_s), r), 1);
+    };
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (uint32_t i = 0; i < ACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16); }
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 for (uint32_t left = k1 - k0; left; --left, ++it) {
                     const CUtensorMap* const ma = &maps.a[p.outs == 2 ? c.z : seg];
                     const CUtensorMap* const mb = &maps.b[GATED ? rank : seg];
-                    if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
+                    if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status, p.polls)) { ok = false; break; }
                     const uint32_t bar = map_to(smem_addr(&full[slot]), lead);          // the leader counts the bytes of both
                     if (rank == 0) mbar_expect(&full[slot], 2 * STAGE);
 #pragma unroll
@@ -298,13 +306,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (++kb == p.kblocks) { kb = 0; ++seg; }
                 }
             }
-            if (!ok) {        // the last copies land before the CTA may end: the leader's barriers count those of both
-                if (rank == 0)
-                    for (uint32_t f = it > STAGES ? it - STAGES : 0; f < it; ++f)
-                        for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&full[f % STAGES], (f / STAGES) & 1); ++i) {}
-                else
-                    for (uint32_t i = 0; i < 2000; ++i) __nanosleep(1000);
-            }
+            for (uint32_t f = it > STAGES ? it - STAGES : 0; ok && f < it; ++f) ok = mbar_wait(&empty[f % STAGES], (f / STAGES) & 1, abort_flag, status, p.polls);
+            issued_s = it;
+            if (!ok) give_up();
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -313,12 +317,12 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             bool ok = true, ready = mbar_test(&full[0], 0);      // a stage ahead: the answer arrives while the products before it are issued
             for (uint32_t t = pair; ok && t < p.tiles; t += pairs, ++n) {
                 const uint32_t buf = n % ACC, acc = tmem + buf * N;
-                if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status)) break;
+                if (n >= ACC && !mbar_wait(&acc_empty[buf], (n / ACC - 1) & 1, abort_flag, status, p.polls)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t more = 0, kb = kb0;
                 for (uint32_t left = k1 - k0; left; --left) {
                     const uint32_t stage = ring + slot * STAGE, now = slot;
-                    if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
+                    if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status, p.polls)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (++slot == STAGES) { slot = 0; phase ^= 1; }
                     ready = mbar_test(&full[slot], phase);
@@ -357,10 +361,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
                 if (ok) umma_commit_pair(&acc_full[buf], lead);
             }
-            if (abort_s) {       // products in flight read shared memory and write tensor memory: they end first
-                umma_commit_pair(&drain, lead);
-                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
-            }
+            if (!ok) give_up();
+            umma_commit_lead(&drain);       // products read shared memory of both CTAs and write their tensor memory
+            mbar_await(&drain, 0);
         }
         __syncwarp();
     } else {
@@ -371,7 +374,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         for (uint32_t t = pair; t < p.tiles; t += pairs, ++n) {
             const Tile c = tile_at(p, t, WIDTH);
             const uint32_t buf = n % ACC, acc = tmem + buf * N + (quarter << 21);
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (n / ACC) & 1, abort_flag, status))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (n / ACC) & 1, abort_flag, status, p.polls))) {
+                if (lane == 0) give_up();
+                break;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float v[COLS], w[GATED ? COLS : 1];
 #pragma unroll
@@ -446,6 +452,19 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (Smem::shared && p.splits > 1) cluster_leave();       // (the arrivals at the leader's barriers came before the sums)
     else cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (*abort_flag) {       // (all CTAs of the cluster or none: the flags were set before their last barrier)
+        if (threadIdx.x == 0 && rank == 0) {      // the leader's barriers count the bytes of both CTAs, which may have started different numbers of stages
+            const uint32_t mine = issued_s, other = load_cluster_word(map_to(smem_addr(&issued_s), lead + 1)), most = max(mine, other);
+            for (uint32_t f = most > STAGES ? most - STAGES : 0; f < most; ++f) {
+                uint64_t* const bar = &full[f % STAGES];
+                if (f >= mine) mbar_expect(bar, STAGE);
+                else if (f >= other) mbar_complete(bar, STAGE);
+                mbar_await(bar, (f / STAGES) & 1);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
@@ -491,7 +510,7 @@ struct FewPlan {
     uint32_t smem;
     uint32_t tmem_columns, sf_column, sf_columns;
     uint32_t prefetch;                  // blocks of K to request into L2 ahead
-    uint32_t idesc, ktiles;
+    uint32_t idesc, ktiles, polls;
     const uint8_t *sfw[2], *sfx;
     const void* x;
     uint64_t x_ld;
@@ -628,7 +647,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
             bool ok = true;
             for (uint32_t k = k0; k < k1; ++k, ++it) {
                 const uint32_t a = ring + slot * p.stage;
-                if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status)) { ok = false; break; }
+                if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, status, p.polls)) { ok = false; break; }
                 const uint32_t atoms = MX4 ? min(2u, p.ktiles - kb * 2) : 0;
                 mbar_expect(&full[slot], MATS * A_BYTES + b_bytes + atoms * 512 * (MATS + (fused ? 0 : 1)));
 #pragma unroll
@@ -648,20 +667,28 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 if (++slot == p.stages) { slot = 0; ++round; }
                 if (++kb == p.kblocks) { kb = 0; ++seg; }
             }
+            const uint32_t last = min(it, p.stages);      // stages not known to be released: from `slot` on in the round before (in the first round from 0)
+            if (!round) slot = 0;
+            for (uint32_t i = 0, at = slot, r = round ? round - 1 : 0; ok && i < last; ++i) {
+                ok = mbar_wait(&empty[at], r & 1, abort_flag, status, p.polls);
+                if (++at == p.stages) { at = 0; ++r; }
+            }
             if (!ok)
-                for (uint32_t f = it > p.stages ? it - p.stages : 0; f < it; ++f)
-                    for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&full[f % p.stages], (f / p.stages) & 1); ++i) {}
+                for (uint32_t i = 0, at = slot, r = round ? round - 1 : 0; i < last; ++i) {
+                    mbar_await(&full[at], r & 1);
+                    if (++at == p.stages) { at = 0; ++r; }
+                }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
-            bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status);
+            bool ok = !fused || mbar_wait(&tokens_ready, 0, abort_flag, status, p.polls);
             uint32_t slot = 0, phase = 0, kb = kb0, more = 0;
             uint32_t quantised = ring + p.resident;
             bool ready = mbar_test(&full[0], 0);
             for (uint32_t k = k0; ok && k < k1; ++k) {
                 const uint32_t a = ring + slot * p.stage, now = slot;
-                if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status)) { ok = false; break; }
+                if (!ready && !mbar_wait(&full[slot], phase, abort_flag, status, p.polls)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (++slot == p.stages) { slot = 0; phase ^= 1; }
                 ready = mbar_test(&full[slot], phase);
@@ -698,11 +725,9 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 if (++kb == p.kblocks) kb = 0;
                 quantised += p.n * 128 + 1024;
             }
-            if (ok) umma_commit(&acc_full);
-            else {
-                umma_commit(&drain);
-                for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(&drain, 0); ++i) {}
-            }
+            uint64_t* const end = ok ? &acc_full : &drain;
+            umma_commit(end);
+            mbar_await(end, 0);
         }
         __syncwarp();
     } else {
@@ -715,7 +740,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
             mbar_arrive(&tokens_ready);
         }
         const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, abort_flag, status));
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, abort_flag, status, p.polls));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         float* const part = reinterpret_cast<float*>(ring_p);        // [matrix][token][row]: every stage has been read when the products are done
         for (uint32_t t0 = 0; ok && t0 < p.tokens; t0 += 16) {
@@ -896,6 +921,7 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     p.aligned = rows16(p.out[0], p.ldo, dtype_bytes(p.out_type)) && p.N * dtype_bytes(p.out_type) % 16 == 0;
     for (int i = 0; i < 3 && p.aligned; ++i)
         if (to[i] && !map_output(maps.o[i], to[i], p.g && i ? p.saved_type : p.out_type, p, GATED ? N / 4 : N / 2)) return no_maps();
+    p.polls = wait_polls.load(std::memory_order_relaxed);
     const uint32_t pairs = d.sms / 2, total = p.segs * p.kblocks;
     // K is shared by four or two pairs where all of the tiles still run at once and it is long enough to pay for the sums: narrow tiles, four pairs
     // from 12 stages on (16-bit 256 x 2048 x 512 8.9 us, shared by none 9.9; of 8 stages 8.3 by two and 7.6), two from 18 (512 x 3000 x 1000 15.1 and
@@ -968,6 +994,7 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
 template <bool MX4, bool A_MN, int MATS> int launch_few(const TileMaps& maps, FewPlan& p, const Device& d, cudaStream_t s) {
     static Configured configured;
     p.out_vec = rows16(p.out, p.ldo, dtype_bytes(p.out_type));
+    p.polls = wait_polls.load(std::memory_order_relaxed);
     auto kernel = few_kernel<MX4, A_MN, MATS>;
     const int rc = configured.once(kernel, d.index, CTA_SMEM_MAX, FEW_THREADS, false);
     if (rc != ZC_OK) return rc;
@@ -1187,6 +1214,12 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
         rc = narrow ? launch_tiles<false, true, true, false, 128>(maps, p, d, s) : launch_tiles<false, true, true, false, 256>(maps, p, d, s);
     }
     return rc;
+}
+
+int zc_ffn_wait_limit(uint32_t polls, uint32_t* before) {
+    const uint32_t old = wait_polls.exchange(polls);
+    if (before) *before = old;
+    return ZC_OK;
 }
 
 int zc_ffn_status(void* stream, uint32_t* status) {

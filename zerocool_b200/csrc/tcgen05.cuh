@@ -40,6 +40,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return false;
 }
 
+// The end of what is in flight already, for a role that is about to leave: bounded, and raises nothing.
+__device__ __forceinline__ void mbar_await(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(bar, parity); ++i) {}
+}
+
 // The same for the lane that feeds the tensor cores: it has nothing else to do, and the wake-up of a suspended wait
 // (a few hundred clocks) is idle tensor time, so it polls without suspending. Still bounded.
 __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t limit = POLL_LIMIT) {
@@ -111,6 +116,9 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void mbar_complete(uint64_t* bar, uint32_t bytes) {      // counts bytes that no copy will bring
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
@@ -160,6 +168,15 @@ __device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t d
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t lead) {      // arrives at this barrier of both CTAs, ranks lead and lead + 1
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"(uint16_t(3u << lead)) : "memory");
 }
+__device__ __forceinline__ void umma_commit_lead(uint64_t* bar) {      // of a pair's products, at this CTA's barrier alone
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t load_cluster_word(uint32_t addr) {      // addresses of map_to
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_cluster_word(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ float load_cluster(uint32_t addr) {      // an address of map_to
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

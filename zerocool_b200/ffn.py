@@ -20,7 +20,7 @@ from . import moe
 from .records import BF16, F16, F32
 
 EXPORTS = ["zc_mx4_scale_bytes", "zc_mx4_quantize", "zc_mx4_dequantize", "zc_mx4_tile_scales", "zc_mx4_linear", "zc_mx4_gated",
-           "zc_gated_forward", "zc_gated_backward", "zc_ffn_status"]
+           "zc_gated_forward", "zc_gated_backward", "zc_ffn_status", "zc_ffn_wait_limit"]
 
 _lib = None
 # torch's handle of the current stream without a Stream object around it (2 us less a call); absent from builds without CUDA.
@@ -42,6 +42,7 @@ def load_library():
         lib.zc_gated_forward.argtypes = [vp, u64, vp, vp, i32, u32, u32, u32, vp, vp, vp, i32, vp]
         lib.zc_gated_backward.argtypes = [vp, u64, vp, u64, vp, vp, vp, vp, i32, i32, u32, u32, u32, vp, vp, vp, vp, vp, vp]
         lib.zc_ffn_status.argtypes = [vp, ctypes.POINTER(u32)]
+        lib.zc_ffn_wait_limit.argtypes = [u32, ctypes.POINTER(u32)]
         _lib = lib
     return _lib
 
@@ -300,3 +301,15 @@ def status(device=None):
     if rc != moe.ZC_OK:
         moe._raise(rc, lib.zc_last_error())
     return word.value
+
+
+WAIT_POLLS = 1 << 20
+
+
+def wait_limit(polls=WAIT_POLLS):
+    """Sets how often a wait inside the products' kernels polls before it gives up (zc_ffn_wait_limit); -> the limit so far."""
+    if isinstance(polls, bool) or not isinstance(polls, int) or not 0 <= polls < 1 << 32:
+        raise ValueError("polls must be a whole number of 32 bits")
+    before = ctypes.c_uint32()
+    load_library().zc_ffn_wait_limit(polls, ctypes.byref(before))
+    return before.value
