@@ -80,7 +80,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
 int zc_ffn_status(void* stream, uint32_t* status);
 
 /* How often a wait inside the products' kernels polls before it gives up, for the calls of this process that follow (a captured call keeps what it was
- * captured with): a poll takes about a microsecond at most. before (may be NULL) receives the limit so far. */
+ * captured with), up to 2^27: a poll takes about a microsecond at most. before (may be NULL) receives the limit so far. */
 #define ZC_FFN_WAIT_POLLS 1048576u   /* the limit that holds until the first such call */
 int zc_ffn_wait_limit(uint32_t polls, uint32_t* before);
 

@@ -132,3 +132,11 @@ def test_arguments_of_the_wrong_kind_are_value_errors(wrong):
                  lambda: ffn.gated_forward(x, wrong, x), lambda: ffn.gated_backward(x, x, wrong, x, x, x)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_wait_limit():
+    assert ffn.wait_limit(5) == ffn.WAIT_POLLS == 1 << 20 and ffn.wait_limit() == 5
+    for wrong in (-1, (1 << 27) + 1, 2.0, None, True):
+        with pytest.raises(ValueError, match="2\\^27"):
+            ffn.wait_limit(wrong)
+    assert ffn.load_library().zc_ffn_wait_limit((1 << 27) + 1, None) == ZC_EINVAL and ffn.wait_limit() == ffn.WAIT_POLLS

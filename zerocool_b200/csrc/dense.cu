@@ -17,7 +17,7 @@
 // Every wait is bounded (POLL_LIMIT polls, unless zc_ffn_wait_limit says otherwise): one that runs out raises ZC_STATUS_TIMEOUT and the abort
 // flag, of both CTAs of a pair and all pairs of a tile; the roles leave their loops, and no CTA frees its tensor memory or ends before the
 // copies and products that it has started have ended. A copy has ended when its stage is released; the copying thread therefore waits for the
-// last stages too (while the others drain the last tile), and where that is cut short, for the bytes themselves.
+// last stage too (while the others drain the last tile), and where that is cut short, for the bytes themselves.
 #include "ffn.cuh"
 #include "tcgen05.cuh"
 #include <atomic>
@@ -242,6 +242,21 @@ template <bool MX4, bool GATED, int N> struct TileSmem {
     static_assert(used <= bytes && bytes <= CTA_SMEM_MAX, "shared memory of a tile CTA");
 };
 
+// The copying thread of a pair's leader, once a wait has run out: the leader's barriers count the bytes of both CTAs, which may have started different
+// numbers of stages, `mine` and what the other CTA's thread leaves in *others, plus one, when it stops. What the other has started alone is expected
+// here, what it has not started is counted off, so that every barrier of the last round flips when its copies have landed. (Without an answer the other
+// has started all, and all of them have been used.) Until the leader is here, neither CTA passes the barrier behind which it ends.
+__device__ __noinline__ void end_copies(uint64_t* full, uint32_t mine, const volatile uint32_t* others, uint32_t stages, uint32_t bytes) {
+    for (uint32_t i = 0; i < POLL_LIMIT && !*others; ++i) {}
+    const uint32_t theirs = *others ? *others - 1 : mine, most = max(mine, theirs);
+    for (uint32_t f = most > stages ? most - stages : 0; f < most; ++f) {
+        uint64_t* const bar = &full[f % stages];
+        if (f >= mine) mbar_expect(bar, bytes);
+        else if (f >= theirs) mbar_complete(bar, bytes);
+        mbar_await(bar, (f / stages) & 1);
+    }
+}
+
 template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const TilePlan p) {
     typedef TileSmem<MX4, GATED, N> Smem;
@@ -250,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     constexpr uint32_t WIDTH = GATED ? N / 2 : N;         // output columns of a tile
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[ACC], acc_empty[ACC], drain;       // (CTA_STATIC bytes at most)
-    __shared__ uint32_t tmem_s, abort_s, issued_s;       // issued_s: the stages that this CTA's copying thread has started
+    __shared__ uint32_t tmem_s, abort_s, others_s;       // others_s: see end_copies
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank() & 1, part = cluster_rank() >> 1, lead = part * 2;            // lead: the leader's rank in the cluster
     const uint32_t pair = cluster_index(), pairs = cluster_count();
@@ -265,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (uint32_t i = 0; i < ACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16); }
         mbar_init(&drain, 1);
-        abort_s = 0;
+        abort_s = others_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -319,9 +334,13 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (++kb == p.kblocks) { kb = 0; ++seg; }
                 }
             }
-            for (uint32_t f = it > STAGES ? it - STAGES : 0; ok && f < it; ++f) ok = mbar_wait(&empty[f % STAGES], (f / STAGES) & 1, abort_flag, status, p.polls);
-            issued_s = it;
-            if (!ok) give_up();
+            const uint32_t last = slot ? slot - 1 : STAGES - 1;
+            if (ok) ok = mbar_spin(&empty[last], (slot ? round : round - 1) & 1, abort_flag, status, p.polls);
+            if (!ok) {
+                give_up();
+                if (rank) store_cluster_word(map_to(smem_addr(&others_s), lead), it + 1);
+                else end_copies(full, it, &others_s, STAGES, STAGE);
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -463,19 +482,6 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     if (Smem::shared && p.splits > 1) cluster_leave();       // (the arrivals at the leader's barriers came before the sums)
     else cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (*abort_flag) {       // (all CTAs of the cluster or none: the flags were set before their last barrier)
-        if (threadIdx.x == 0 && rank == 0) {      // the leader's barriers count the bytes of both CTAs, which may have started different numbers of stages
-            const uint32_t mine = issued_s, other = load_cluster_word(map_to(smem_addr(&issued_s), lead + 1)), most = max(mine, other);
-            for (uint32_t f = most > STAGES ? most - STAGES : 0; f < most; ++f) {
-                uint64_t* const bar = &full[f % STAGES];
-                if (f >= mine) mbar_expect(bar, STAGE);
-                else if (f >= other) mbar_complete(bar, STAGE);
-                mbar_await(bar, (f / STAGES) & 1);
-            }
-        }
-        __syncwarp();
-        cluster_sync();
-    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
@@ -673,17 +679,10 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                 if (++slot == p.stages) { slot = 0; ++round; }
                 if (++kb == p.kblocks) { kb = 0; ++seg; }
             }
-            const uint32_t last = min(it, p.stages);      // stages not known to be released: from `slot` on in the round before (in the first round from 0)
-            if (!round) slot = 0;
-            for (uint32_t i = 0, at = slot, r = round ? round - 1 : 0; ok && i < last; ++i) {
-                ok = mbar_wait(&empty[at], r & 1, abort_flag, status, p.polls);
-                if (++at == p.stages) { at = 0; ++r; }
-            }
+            const uint32_t last = slot ? slot - 1 : p.stages - 1;
+            if (ok) ok = mbar_spin(&empty[last], (slot ? round : round - 1) & 1, abort_flag, status, p.polls);
             if (!ok)
-                for (uint32_t i = 0, at = slot, r = round ? round - 1 : 0; i < last; ++i) {
-                    mbar_await(&full[at], r & 1);
-                    if (++at == p.stages) { at = 0; ++r; }
-                }
+                for (uint32_t f = it > p.stages ? it - p.stages : 0; f < it; ++f) mbar_await(&full[f % p.stages], (f / p.stages) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -1244,6 +1243,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
 }
 
 int zc_ffn_wait_limit(uint32_t polls, uint32_t* before) {
+    if (polls > 1u << 27) return fail(nullptr, ZC_EINVAL, "zc_ffn_wait_limit: more than 2^27 polls");
     const uint32_t old = wait_polls.exchange(polls);
     if (before) *before = old;
     return ZC_OK;

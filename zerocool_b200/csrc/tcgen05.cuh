@@ -40,9 +40,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return false;
 }
 
-// The end of what is in flight already, for a role that is about to leave: bounded, and raises nothing.
+// The end of what is in flight already, for a role that is about to leave: bounded, and raises nothing. Polled, as the others may be waiting
+// for the role at their last barrier (suspended, MX4 8192 x 4096, one token 6.3 us, polled 6.2).
 __device__ __forceinline__ void mbar_await(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < POLL_LIMIT && !mbar_try(bar, parity); ++i) {}
+    for (uint32_t i = 0; i < POLL_LIMIT << 4 && !mbar_test(bar, parity); ++i) {}
 }
 
 // The same for the lane that feeds the tensor cores: it has nothing else to do, and the wake-up of a suspended wait
@@ -171,12 +172,9 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t lead) {
 __device__ __forceinline__ void umma_commit_lead(uint64_t* bar) {      // of a pair's products, at this CTA's barrier alone
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ uint32_t load_cluster_word(uint32_t addr) {      // addresses of map_to
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void store_cluster_word(uint32_t addr, uint32_t v) {      // an address of map_to
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-__device__ __forceinline__ void store_cluster_word(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ float load_cluster(uint32_t addr) {      // an address of map_to
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

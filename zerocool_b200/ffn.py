@@ -308,8 +308,8 @@ WAIT_POLLS = 1 << 20
 
 def wait_limit(polls=WAIT_POLLS):
     """Sets how often a wait inside the products' kernels polls before it gives up (zc_ffn_wait_limit); -> the limit so far."""
-    if isinstance(polls, bool) or not isinstance(polls, int) or not 0 <= polls < 1 << 32:
-        raise ValueError("polls must be a whole number of 32 bits")
+    if isinstance(polls, bool) or not isinstance(polls, int) or not 0 <= polls <= 1 << 27:
+        raise ValueError("polls must be a whole number up to 2^27")
     before = ctypes.c_uint32()
     load_library().zc_ffn_wait_limit(polls, ctypes.byref(before))
     return before.value
