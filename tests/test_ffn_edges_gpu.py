@@ -120,3 +120,25 @@ def test_waits_that_run_out_somewhere(ffn, short_waits, polls):
             short_waits()
             assert gave_up in (0, 2) and (gave_up or torch.equal(got, want)), i
         assert torch.equal(call(), want) and ffn.status() == 0, i
+
+
+# -- clusters that add their sums ----------------------------------------------------------------------------------------------
+
+def test_sums_of_ragged_tiles_while_clusters_come_and_go(ffn):
+    """Tiles of which most rows lie past the matrix, their K split over clusters of up to eight CTAs, on three streams at once: clusters start and end
+    beside one another all the time, and every result is that of the call alone."""
+    jobs = []
+    for rows in (1, 5, 130, 200, 259):
+        w = [ffn.mx4_quantize(randn((rows, 2080), 10 + i, 0.1)) for i in range(2)]
+        for tokens in (1, 3, 33, 130, 260):
+            x = randn((tokens, 2080), tokens, dtype=torch.bfloat16)
+            jobs += [lambda x=x, w=w: ffn.mx4_linear(x, w[0]), lambda x=x, w=w: ffn.mx4_gated(x, *w)]
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for round_ in range(6):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[(i + round_) % 3]):
+                got.append((i, job()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)

@@ -453,7 +453,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 uint8_t* const patch = raw + (ring - smem_addr(raw)) + STAGES * STAGE + (warp - 2) * Smem::patch;
                 const Tile c = tile_at(p, pair, WIDTH);
                 const uint32_t row = c.m0 + rank * TILE_M + quarter * 32;
-                for (uint32_t j = part * share + ((warp - 2) >> 2) * 8; j < (part + 1) * share; j += 16) {
+                // A warp without rows loads nothing, the others use all that they load: cluster_leave waits for no load.
+                const uint32_t end = row < p.M ? (part + 1) * share : 0;
+                for (uint32_t j = part * share + ((warp - 2) >> 2) * 8; j < end; j += 16) {
                     float v[8], w[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = w[i] = 0.0f;
@@ -793,8 +795,9 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
     if (p.splits > 1) {
-        if (warp >= 2 && !*abort_flag) {
-            const uint32_t row = lane * 4;           // four rows a lane, a token a warp
+        // Sums that are not stored are not loaded either: cluster_leave waits for no load, so each of them has to be used before it.
+        const uint32_t row = lane * 4;               // four rows a lane, a token a warp
+        if (warp >= 2 && m0 + row < p.M && !*abort_flag) {
             for (uint32_t t = rank + (warp - 2) * p.splits; t < p.tokens; t += 4 * p.splits) {
                 float4 v[MATS];
 #pragma unroll
@@ -808,7 +811,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
                     for (uint32_t r = 1; r < 8; ++r)
                         if (r < p.splits) { v[i].x += each[r].x; v[i].y += each[r].y; v[i].z += each[r].z; v[i].w += each[r].w; }
                 }
-                few_store4<MATS == 2>(p, uint64_t(t) * p.ldo + m0 + row, m0 + row < p.M ? p.M - m0 - row : 0, v[0], v[MATS - 1]);
+                few_store4<MATS == 2>(p, uint64_t(t) * p.ldo + m0 + row, p.M - m0 - row, v[0], v[MATS - 1]);
             }
         }
         __syncwarp();

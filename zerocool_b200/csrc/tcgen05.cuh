@@ -131,7 +131,8 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {      
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
     return there;
 }
-// The same for CTAs that have only loaded from one another (and hold what they loaded): nothing is handed over, so no earlier store is waited for.
+// The same for CTAs that have only loaded from one another: nothing is handed over, so no earlier store is waited for, and no earlier load either. Every
+// value that was loaded has to be used by a store to memory before it: until then a load may be under way to a CTA that this barrier lets end.
 __device__ __forceinline__ void cluster_leave() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
