@@ -7,7 +7,7 @@
  *  - Plain C: ZC_OK or a negative code; zc_last_error() has the text. Everything is validated on the host before a launch.
  *  - No handle and no allocation: every buffer is the caller's device memory, on the current device, 16-byte aligned. Calls are
  *    stream-ordered, do not block the host and may be captured into a graph (make one call of an entry point before its first capture,
- *    which loads its kernels). Calls on different streams share nothing.
+ *    which loads its kernels). Calls on different streams share nothing but the status word of the device.
  *  - Zero tokens (rows) is a valid call: nothing is read or written, but that gradients of the weights become zero.
  *  - Results do not depend on what else runs and are the same bits on every call: no atomics, a fixed order of sums.
  *  - A wait inside a kernel is bounded (zc_ffn_wait_limit); one that runs out raises ZC_STATUS_TIMEOUT in a word of the device (zc_ffn_status).
@@ -76,7 +76,8 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
 int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_ld, const void* gate, const void* up, const void* g, const void* u,
                       int saved_dtype, int dtype, uint32_t tokens, uint32_t hidden, uint32_t ffn, void* dg, void* du, void* dx, void* dgate, void* dup, void* stream);
 
-/* Waits for `stream` and returns the current device's status word of these operators (then clears it). */
+/* Waits for `stream` and returns the current device's status word of these operators (then clears it). The word is that of all streams of the device: a
+ * call may return, and clear, a time-out of another stream's kernels; none is cleared that no call returned. */
 int zc_ffn_status(void* stream, uint32_t* status);
 
 /* How often a wait inside the products' kernels polls before it gives up, for the calls of this process that follow (a captured call keeps what it was

@@ -122,6 +122,28 @@ def test_waits_that_run_out_somewhere(ffn, short_waits, polls):
         assert torch.equal(call(), want) and ffn.status() == 0, i
 
 
+def test_no_time_out_is_cleared_unseen(ffn, short_waits):
+    """Time-outs raised on one stream at every moment of a status call on another: the call returns it, or the next one does."""
+    x, w = randn((1, 256), 1, dtype=torch.bfloat16), ffn.mx4_quantize(randn((128, 256), 2))
+    ffn.mx4_linear(x, w)
+    raising, asking = torch.cuda.Stream(), torch.cuda.Stream()
+    late = torch.zeros(600 << 17, device="cuda")
+    torch.cuda.synchronize()
+    lost = 0
+    for i in range(600):
+        with torch.cuda.stream(raising):
+            late[:i << 17].add_(1.0)             # up to 100 us and more: the call below meets the time-out at another moment each time
+            short_waits(0)
+            ffn.mx4_linear(x, w)
+            short_waits()
+        with torch.cuda.stream(asking):
+            seen = ffn.status()
+        raising.synchronize()
+        seen |= ffn.status()
+        lost += seen != 2
+    assert lost == 0
+
+
 # -- clusters that add their sums ----------------------------------------------------------------------------------------------
 
 def test_sums_of_ragged_tiles_while_clusters_come_and_go(ffn):

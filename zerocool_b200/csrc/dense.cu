@@ -1257,8 +1257,13 @@ int zc_ffn_status(void* stream, uint32_t* status) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint32_t zero = 0;
     cudaError_t e = cudaMemcpyFromSymbolAsync(status, ffn_status_word, 4, 0, cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(ffn_status_word, &zero, 4, 0, cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    // Cleared only where it was found set: what another stream raises after the read is then either left in the word, or the same bit as the one that
+    // this call returns. (Its only bit is ZC_STATUS_TIMEOUT.)
+    if (e == cudaSuccess && *status) {
+        e = cudaMemcpyToSymbolAsync(ffn_status_word, &zero, 4, 0, cudaMemcpyHostToDevice, s);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    }
     if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("status: ") + cudaGetErrorString(e)); }
     return ZC_OK;
 }

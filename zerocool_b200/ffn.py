@@ -293,7 +293,7 @@ def gated_backward(dh, x, gate, up, g, u, input_grad=True, weight_grads=True):
 
 
 def status(device=None):
-    """Waits for the device's current stream and returns (then clears) the device's status word of these operators."""
+    """Waits for the device's current stream and returns (then clears) the device's status word of these operators, the same for all of its streams."""
     word = ctypes.c_uint32()
     lib = load_library()
     with torch.cuda.device(device):
