@@ -140,3 +140,9 @@ def test_wait_limit():
         with pytest.raises(ValueError, match="2\\^27"):
             ffn.wait_limit(wrong)
     assert ffn.load_library().zc_ffn_wait_limit((1 << 27) + 1, None) == ZC_EINVAL and ffn.wait_limit() == ffn.WAIT_POLLS
+
+
+@pytest.mark.parametrize("rows,cols,device", [(4, 64, "cpu"), (4, 64, "meta"), (0, 32, "cpu"), (-1, 64, "cuda"), (4, 48, "cuda"), (4, 0, "cuda"), (4.0, 64, "cuda"), (4, None, "cuda")])
+def test_matrices_yet_to_be_written_are_on_a_cuda_device(rows, cols, device):
+    with pytest.raises(ValueError):
+        ffn.Mx4.empty(rows, cols, device)

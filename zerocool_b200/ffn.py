@@ -156,10 +156,13 @@ class Mx4:
 
     @staticmethod
     def empty(rows, cols, device):
-        if cols <= 0 or cols % 32:
-            raise ValueError("columns must be a multiple of 32")
+        """A matrix whose values are yet to be written (mx4_quantize(..., out=))."""
+        if not isinstance(rows, int) or not isinstance(cols, int) or rows < 0 or cols <= 0 or cols % 32:
+            raise ValueError("rows and columns must be whole numbers, columns a multiple of 32")
         q = object.__new__(Mx4)          # nothing to check
         q.codes = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
+        if not q.codes.is_cuda:
+            raise ValueError("the device must be a CUDA device")
         q.scales = q.codes.new_empty(_scale_bytes(rows, cols))
         return q
 
