@@ -9,7 +9,7 @@ import torch
 
 from tests import mx4_reference as ref
 from zerocool_b200 import ffn
-from zerocool_b200.moe import ZC_EINVAL, ZC_OK
+from zerocool_b200.moe import ZC_EEXEC, ZC_EINVAL, ZC_OK
 from zerocool_b200.records import BF16, F16, F32
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -146,3 +146,16 @@ def test_wait_limit():
 def test_matrices_yet_to_be_written_are_on_a_cuda_device(rows, cols, device):
     with pytest.raises(ValueError):
         ffn.Mx4.empty(rows, cols, device)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a call that is not refused ends for want of a device")
+@pytest.mark.parametrize("x,x_dtype,out,out_dtype,ld,apart", [
+    (0, F32, 64, F32, 72, True), (8, F32, 0, F32, 72, True), (0, F32, 64, F32, 73, True), (0, F32, 63, F32, 72, False), (7, F32, 0, F32, 72, False),
+    (0, F32, 64, F32, 71, False), (72, F32, 64, F32, 72, True), (72, F32, 63, F32, 72, False), (0, F32, 64 + 3 * 72, F32, 72, True), (0, F32, 62 + 3 * 72, F32, 72, False),
+])
+def test_columns_of_one_buffer_side_by_side(x, x_dtype, out, out_dtype, ld, apart):
+    """x (64 columns) and out (8) of four rows in one buffer, their first elements at these places: refused only where they share an element."""
+    rc = linear(x=at(7) + 4 * x, x_dtype=x_dtype, x_ld=ld, out=at(7) + 4 * out, out_dtype=out_dtype, out_ld=ld)
+    rows = lambda first, n: {first + r * ld + c for r in range(4) for c in range(n)}  # noqa: E731
+    assert apart == (not rows(x, 64) & rows(out, 8))
+    assert rc == (ZC_EEXEC if apart else ZC_EINVAL) and (b"overlapping" in ffn.load_library().zc_last_error()) != apart

@@ -164,3 +164,20 @@ def test_sums_of_ragged_tiles_while_clusters_come_and_go(ffn):
                 got.append((i, job()))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i, y in got)
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 60, 300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_x_and_result_side_by_side_in_one_buffer(ffn, tokens, dtype):
+    """x and the results of two products as columns of one buffer, of aligned and of odd row strides: every column keeps what belongs to it."""
+    w, v = ffn.mx4_quantize(randn((200, 320), 1, 0.1)), ffn.mx4_quantize(randn((200, 320), 2, 0.1))
+    x = randn((tokens, 320), 3, dtype=dtype)
+    for gap in (0, 1, 8):
+        buffer = torch.full((tokens, 720 + 2 * gap), 7.0, dtype=dtype, device="cuda")
+        left, mid, right = buffer[:, :200], buffer[:, 200 + gap:520 + gap], buffer[:, 520 + 2 * gap:]
+        mid.copy_(x)
+        ffn.mx4_linear(mid, w, out=left)
+        ffn.mx4_gated(mid, w, v, out=right)
+        assert torch.equal(left, ffn.mx4_linear(x, w, dtype)) and torch.equal(right, ffn.mx4_gated(x, w, v, dtype)) and torch.equal(mid, x)
+        with pytest.raises(ValueError, match="overlapping"):
+            ffn.mx4_linear(mid, w, out=buffer[:, 1 + gap:201 + gap])

@@ -1041,8 +1041,8 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     if (rc == ZC_OK && !rows) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": no rows in the weights");
     if (rc == ZC_OK) rc = check_matrix((std::string(who) + ": output").c_str(), out, out_dtype, tokens, rows, out_ld, false);
     if (rc != ZC_OK || !tokens) return rc;
-    const Span os{out, matrix_bytes(out_dtype, tokens, rows, out_ld)}, cs{x_codes, uint64_t(tokens) * cols / 2}, ss{x_scales, mx4_scale_bytes(tokens, cols)};
-    const Span xs{x, x ? matrix_bytes(x_dtype, tokens, cols, x_ld) : 0};
+    const Span os = matrix_span(out, out_dtype, tokens, rows, out_ld), cs{x_codes, uint64_t(tokens) * cols / 2}, ss{x_scales, mx4_scale_bytes(tokens, cols)};
+    const Span xs = x ? matrix_span(x, x_dtype, tokens, cols, x_ld) : Span{nullptr, 0};
     bool bad = overlap(os, cs) || overlap(os, ss) || overlap(os, xs) || (x && (overlap(cs, ss) || overlap(cs, xs) || overlap(ss, xs)));
     for (int i = 0; i < mats; ++i)
         for (const Span& t : {Span{w[i].codes, uint64_t(rows) * cols / 2}, Span{w[i].scales, mx4_scale_bytes(rows, cols)}})

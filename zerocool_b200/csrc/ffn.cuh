@@ -68,13 +68,21 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p
 // ---------------------------------------------------------------------------------------------
 // Arguments
 // ---------------------------------------------------------------------------------------------
-struct Span { const void* p; uint64_t bytes; };
+struct Span { const void* p; uint64_t bytes; uint64_t width = 0, pitch = 0; };      // a matrix of several rows: bytes of a row, and from one to the next
+// Columns side by side in the rows of one buffer share no byte, though the one's rows lie between the other's.
 inline bool overlap(const Span& a, const Span& b) {
-    const char *x = static_cast<const char*>(a.p), *y = static_cast<const char*>(b.p);
-    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    if (!a.p || !b.p || !a.bytes || !b.bytes || x >= y + b.bytes || y >= x + a.bytes) return false;
+    const uint64_t pitch = a.pitch ? a.pitch : b.pitch;
+    if (!pitch || (a.pitch && b.pitch && a.pitch != b.pitch)) return true;
+    const uint64_t after = x >= y ? (x - y) % pitch : (pitch - (y - x) % pitch) % pitch;      // where a row of a starts, from the start of b's row before it
+    return after < (b.pitch ? b.width : b.bytes) || after + (a.pitch ? a.width : a.bytes) > pitch;
 }
 inline uint64_t dtype_bytes(int dtype) { return dtype == ZC_F32 ? 4 : 2; }
 inline uint64_t matrix_bytes(int dtype, uint64_t rows, uint64_t cols, uint64_t ld) { return rows ? ((rows - 1) * ld + cols) * dtype_bytes(dtype) : 0; }
+inline Span matrix_span(const void* p, int dtype, uint64_t rows, uint64_t cols, uint64_t ld) {
+    return rows > 1 ? Span{p, matrix_bytes(dtype, rows, cols, ld), cols * dtype_bytes(dtype), ld * dtype_bytes(dtype)} : Span{p, matrix_bytes(dtype, rows, cols, ld)};
+}
 inline bool misaligned(const void* p, uintptr_t to = 16) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 // Whether every row of a matrix starts on 16 bytes.
 inline bool rows16(const void* p, uint64_t ld, uint64_t elem) { return !misaligned(p) && ld * elem % 16 == 0; }
