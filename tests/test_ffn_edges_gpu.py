@@ -181,3 +181,22 @@ def test_x_and_result_side_by_side_in_one_buffer(ffn, tokens, dtype):
         assert torch.equal(left, ffn.mx4_linear(x, w, dtype)) and torch.equal(right, ffn.mx4_gated(x, w, v, dtype)) and torch.equal(mid, x)
         with pytest.raises(ValueError, match="overlapping"):
             ffn.mx4_linear(mid, w, out=buffer[:, 1 + gap:201 + gap])
+
+
+def test_operands_that_require_gradients(ffn):
+    """Where gradients are recorded a result without one is refused; without recording the call is as ever, and gated_backward gives the gradients."""
+    x, gate, up = (randn((r, 64), s, dtype=torch.bfloat16) for s, r in ((1, 5), (2, 16), (3, 16)))
+    w = ffn.mx4_quantize(gate.requires_grad_())                     # codes have no gradient: nothing is lost
+    want = ffn.gated_forward(x, gate.detach(), up)
+    for call in (lambda: ffn.gated_forward(x, gate, up), lambda: ffn.gated_forward(x.clone().requires_grad_(), gate.detach(), up, save=True),
+                 lambda: ffn.gated_forward(x, gate.detach(), up.clone().requires_grad_()), lambda: ffn.mx4_linear(x.clone().requires_grad_(), w),
+                 lambda: ffn.mx4_gated(x.clone().requires_grad_(), w, w)):
+        with pytest.raises(ValueError, match="autograd"):
+            call()
+    with torch.no_grad():
+        h, g, u = ffn.gated_forward(x, gate, up, save=True)
+        assert torch.equal(h, want)
+    dx, dgate, dup = ffn.gated_backward(torch.ones_like(h), x, gate, up, g, u)
+    assert not (dx.requires_grad or dgate.requires_grad or dup.requires_grad)
+    with torch.inference_mode():
+        assert torch.equal(ffn.mx4_linear(x, w), ffn.mx4_linear(x.detach(), w))

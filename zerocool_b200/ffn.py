@@ -9,8 +9,9 @@ its gradient - the shared or dense form of the block whose routed form is ``zero
     dx, dgate, dup = gated_backward(dh, x, gate, up, g, u)
 
 Calls run on the tensors' device and torch's current stream of it, allocate results and scratch with torch and may be captured into a
-CUDA graph (after one call outside a capture). Nothing here has a CPU path, and autograd does not see these calls. Errors are those of ``zerocool_b200.moe``: ``ValueError``
-for arguments, ``RuntimeError`` for the device.
+CUDA graph (after one call outside a capture). Nothing here has a CPU path, and autograd does not see these calls: a block or product of tensors that
+require gradients is refused where gradients are recorded, as its result would silently have none (call it under ``torch.no_grad()``, or pass
+``x.detach()``). Errors are those of ``zerocool_b200.moe``: ``ValueError`` for arguments, ``RuntimeError`` for the device.
 """
 import ctypes
 
@@ -81,6 +82,12 @@ def _whole(name, t, shape, dtype, device):
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
         _matrix(name, t, shape, dtype, contiguous=True)
         _same_device(device, **{name: t})
+
+
+def _unrecorded():
+    """For operands that require gradients."""
+    if torch.is_grad_enabled():
+        raise ValueError("autograd does not see this call: its result would not have the gradient that its operands require (torch.no_grad(), or detach them)")
 
 
 def _tensor(name, t):
@@ -220,6 +227,8 @@ def _mx4_product(entry, x, weights, out_dtype, out):
         codes, scales = x.codes.data_ptr(), x.scales.data_ptr()
     else:
         ld = _matrix("x", x)
+        if x.requires_grad:
+            _unrecorded()
         (tokens, xcols), plain = x.shape, (x.data_ptr(), _code(x.dtype), ld)
         scratch = torch.empty(tokens * cols // 2 + _scale_bytes(tokens, cols), dtype=torch.uint8, device=device)      # codes, then scales
         codes = scratch.data_ptr()
@@ -256,6 +265,8 @@ def gated_forward(x, gate, up, save=False, save_dtype=torch.float32, out=None):
     dtype, device = x.dtype, x.device
     _whole("gate", gate, (ffn, hidden), dtype, device)
     _whole("up", up, (ffn, hidden), dtype, device)
+    if x.requires_grad or gate.requires_grad or up.requires_grad:
+        _unrecorded()
     if out is None:
         out = x.new_empty((tokens, ffn))
     else:
