@@ -159,3 +159,15 @@ def test_columns_of_one_buffer_side_by_side(x, x_dtype, out, out_dtype, ld, apar
     rows = lambda first, n: {first + r * ld + c for r in range(4) for c in range(n)}  # noqa: E731
     assert apart == (not rows(x, 64) & rows(out, 8))
     assert rc == (ZC_EEXEC if apart else ZC_EINVAL) and (b"overlapping" in ffn.load_library().zc_last_error()) != apart
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a call that is not refused ends for want of a device")
+@pytest.mark.parametrize("ld", [0, 8, 20, 1 << 40])
+def test_the_stride_of_a_single_row_is_not_looked_at(ld):
+    for call in (lambda: forward(tokens=1, x_ld=ld), lambda: backward(tokens=1, dh_ld=ld, x_ld=ld), lambda: linear(x=at(7), x_ld=ld, tokens=1, out_ld=ld), lambda: quantize(rows=1, ld=ld)):
+        assert call() == ZC_EEXEC
+
+
+def test_strides_of_several_rows_are():
+    for ld in (0, 8, 20, 1 << 40):
+        assert forward(tokens=2, x_ld=ld) == ZC_EINVAL and backward(tokens=2, x_ld=ld) == ZC_EINVAL and quantize(rows=2, ld=ld) == ZC_EINVAL

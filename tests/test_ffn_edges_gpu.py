@@ -200,3 +200,17 @@ def test_operands_that_require_gradients(ffn):
     assert not (dx.requires_grad or dgate.requires_grad or dup.requires_grad)
     with torch.inference_mode():
         assert torch.equal(ffn.mx4_linear(x, w), ffn.mx4_linear(x.detach(), w))
+
+
+@pytest.mark.parametrize("ld", [0, 8, 20, 1 << 40])
+def test_a_single_row_of_any_stride(ffn, ld):
+    x, gate, up = (randn((r, 64), s, dtype=torch.bfloat16) for s, r in ((1, 1), (2, 16), (3, 16)))
+    h, g, u = torch.empty(1, 16, dtype=torch.bfloat16, device="cuda"), torch.empty(1, 16, device="cuda"), torch.empty(1, 16, device="cuda")
+    code, stream = ffn.CODES[torch.bfloat16], torch.cuda.current_stream().cuda_stream
+    assert ffn.load_library().zc_gated_forward(x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), code, 1, 64, 16, h.data_ptr(), g.data_ptr(), u.data_ptr(), ffn.CODES[torch.float32], stream) == 0
+    assert all(torch.equal(a, b) for a, b in zip((h, g, u), ffn.gated_forward(x, gate, up, save=True)))
+    got, want = torch.empty_like(up), ffn.gated_backward(h, x, gate, up, g, u)
+    dg, du, dx, dgate = torch.empty_like(h), torch.empty_like(h), torch.empty_like(x), torch.empty_like(gate)
+    assert ffn.load_library().zc_gated_backward(h.data_ptr(), ld, x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), ffn.CODES[torch.float32], code, 1, 64, 16,
+                                                dg.data_ptr(), du.data_ptr(), dx.data_ptr(), dgate.data_ptr(), got.data_ptr(), stream) == 0
+    assert torch.equal(dx, want[0]) and torch.equal(dgate, want[1]) and torch.equal(got, want[2])

@@ -39,11 +39,11 @@ int check_matrix(const char* who, const void* p, int dtype, uint32_t rows, uint3
     if (dtype != ZC_BF16 && dtype != ZC_F16 && (dtype != ZC_F32 || tma)) return bad(tma ? "dtype must be BF16 or F16" : "dtype must be BF16, F16 or F32");
     if (!cols || rows > 0x7fffffffu) return bad("invalid shape");
     if (rows > 1 && ld < cols) return bad("row stride below the row's length");
-    if (ld > (1ull << 30)) return bad("row stride above 2^30");
+    if (rows > 1 && ld > (1ull << 30)) return bad("row stride above 2^30");
     if (!rows) return ZC_OK;
     if (!p) return bad("missing buffer");
     if (misaligned(p, tma ? 16 : dtype_bytes(dtype))) return bad(tma ? "buffers must be 16-byte aligned" : "buffer is not aligned to its elements");
-    if (tma && ld * dtype_bytes(dtype) % 16) return bad("row stride must be a multiple of 16 bytes");
+    if (tma && rows > 1 && ld * dtype_bytes(dtype) % 16) return bad("row stride must be a multiple of 16 bytes");
     return ZC_OK;
 }
 
@@ -1041,6 +1041,7 @@ int mx4_product(const char* who, const void* x, int x_dtype, uint64_t x_ld, void
     if (rc == ZC_OK && !rows) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": no rows in the weights");
     if (rc == ZC_OK) rc = check_matrix((std::string(who) + ": output").c_str(), out, out_dtype, tokens, rows, out_ld, false);
     if (rc != ZC_OK || !tokens) return rc;
+    if (tokens == 1) { x_ld = cols; out_ld = rows; }
     const Span os = matrix_span(out, out_dtype, tokens, rows, out_ld), cs{x_codes, uint64_t(tokens) * cols / 2}, ss{x_scales, mx4_scale_bytes(tokens, cols)};
     const Span xs = x ? matrix_span(x, x_dtype, tokens, cols, x_ld) : Span{nullptr, 0};
     bool bad = overlap(os, cs) || overlap(os, ss) || overlap(os, xs) || (x && (overlap(cs, ss) || overlap(cs, xs) || overlap(ss, xs)));
@@ -1130,6 +1131,7 @@ int zc_gated_forward(const void* x, uint64_t x_ld, const void* gate, const void*
     if (rc == ZC_OK && tokens && !g != !u) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": g and u go together");
     if (rc == ZC_OK && (g || u)) rc = check_saved(who, g, u, dtype, saved_dtype);
     if (rc != ZC_OK || !tokens) return rc;
+    if (tokens == 1) x_ld = hidden;
     const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2, ts = uint64_t(tokens) * ffn * dtype_bytes(saved_dtype);
     const Span in[3] = {{x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}}, to[3] = {{h, tf}, {g, ts}, {u, ts}};
     for (int i = 0; i < 3; ++i) {
@@ -1176,6 +1178,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     if (rc == ZC_OK && !dgate != !dup) rc = fail(nullptr, ZC_EINVAL, std::string(who) + ": dgate and dup go together");
     for (const void* v : {dgate, dup}) if (rc == ZC_OK && v) rc = check_matrix(who, v, dtype, ffn, hidden, hidden, true);
     if (rc != ZC_OK) return rc;
+    if (tokens == 1) { x_ld = hidden; dh_ld = ffn; }
     const uint64_t tf = uint64_t(tokens) * ffn * 2, fh = uint64_t(ffn) * hidden * 2, th = uint64_t(tokens) * hidden * 2, ts = uint64_t(tokens) * ffn * dtype_bytes(saved_dtype);
     const Span in[6] = {{dh, matrix_bytes(dtype, tokens, ffn, dh_ld)}, {x, matrix_bytes(dtype, tokens, hidden, x_ld)}, {gate, fh}, {up, fh}, {g, ts}, {u, ts}};
     const Span to[5] = {{dg, tf}, {du, tf}, {dx, th}, {dgate, fh}, {dup, fh}};

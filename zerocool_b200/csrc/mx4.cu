@@ -126,6 +126,7 @@ int zc_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint
     if (rc == ZC_OK) rc = check_matrix("zc_mx4_quantize: x", x, dtype, rows, cols, ld, false);
     if (rc != ZC_OK) return rc;
     if (!rows) return ZC_OK;
+    if (rows == 1) ld = cols;
     const Span xs{x, matrix_bytes(dtype, rows, cols, ld)}, cs{codes, uint64_t(rows) * cols / 2}, ss{scales, mx4_scale_bytes(rows, cols)};
     if (overlap(cs, xs) || overlap(ss, xs) || overlap(cs, ss)) return fail(nullptr, ZC_EINVAL, "zc_mx4_quantize: overlapping buffers");
     return launch_mx4_quantize(x, dtype, rows, cols, ld, codes, scales, static_cast<cudaStream_t>(stream));
@@ -136,6 +137,7 @@ int zc_mx4_dequantize(const void* codes, const void* scales, uint32_t rows, uint
     if (rc == ZC_OK) rc = check_matrix("zc_mx4_dequantize: out", out, dtype, rows, cols, ld, false);
     if (rc != ZC_OK) return rc;
     if (!rows) return ZC_OK;
+    if (rows == 1) ld = cols;
     const Span os{out, matrix_bytes(dtype, rows, cols, ld)}, cs{codes, uint64_t(rows) * cols / 2}, ss{scales, mx4_scale_bytes(rows, cols)};
     if (overlap(cs, os) || overlap(ss, os)) return fail(nullptr, ZC_EINVAL, "zc_mx4_dequantize: overlapping buffers");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
