@@ -6,8 +6,8 @@
  * Conventions (those of zc_moe.h where not stated here)
  *  - Plain C: ZC_OK or a negative code; zc_last_error() has the text. Everything is validated on the host before a launch.
  *  - No handle and no allocation: every buffer is the caller's device memory, on the current device, 16-byte aligned. Calls are
- *    stream-ordered, do not block the host and may be captured into a graph (make one call of an entry point before its first capture,
- *    which loads its kernels). Calls on different streams share nothing but the status word of the device.
+ *    stream-ordered, do not block the host and may be captured into a graph (a process's first call of an entry point too: an entry point has
+ *    kernels of several sizes and types, and what a capture meets first is loaded then). Calls on different streams share nothing but the status word of the device.
  *  - Row strides count elements; that of a single row has no meaning and may be anything.
  *  - What a call writes shares no memory with what it reads, or the call is refused; columns side by side in the rows of one buffer share none.
  *  - Zero tokens (rows) is a valid call: nothing is read or written, but that gradients of the weights become zero.

@@ -1,6 +1,9 @@
 """Dense feed-forward operators on the GPU where their arithmetic, their plans and their arguments end (definitions: tests/mx4_reference.py;
 the tolerances are those of tests/test_ffn_gpu.py, and what a test adds to them stands beside it)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -9,6 +12,7 @@ from tests import mx4_reference as ref
 from tests.test_ffn_gpu import HALF, TINY, close, ffn, gen, randn, sums, view_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 FAR = (0.0, 4.0, 16.0, 21.0, 24.0, 28.0, 32.0, 36.0, 48.0, 96.0)
 
@@ -214,3 +218,48 @@ def test_a_single_row_of_any_stride(ffn, ld):
     assert ffn.load_library().zc_gated_backward(h.data_ptr(), ld, x.data_ptr(), ld, gate.data_ptr(), up.data_ptr(), g.data_ptr(), u.data_ptr(), ffn.CODES[torch.float32], code, 1, 64, 16,
                                                 dg.data_ptr(), du.data_ptr(), dx.data_ptr(), dgate.data_ptr(), got.data_ptr(), stream) == 0
     assert torch.equal(dx, want[0]) and torch.equal(dgate, want[1]) and torch.equal(got, want[2])
+
+
+# -- captures ------------------------------------------------------------------------------------------------------------------
+
+CAPTURES = """
+import sys, torch
+from zerocool_b200 import ffn
+first, tokens = sys.argv[1] == "first", int(sys.argv[2])
+torch.manual_seed(0)
+x, dh = torch.randn(tokens, 512, device="cuda").bfloat16(), torch.randn(tokens, 296, device="cuda").bfloat16()
+w, g, u = torch.randn(296, 512, device="cuda").bfloat16(), torch.randn(tokens, 296, device="cuda"), torch.randn(tokens, 296, device="cuda")
+codes, rows = torch.randint(0, 256, (296, 256), device="cuda").to(torch.uint8), torch.randint(100, 130, (296, 16), device="cuda").to(torch.uint8)
+scales = torch.randint(100, 130, (3 * 4 * 512,), device="cuda").to(torch.uint8)
+q = ffn.Mx4(codes, scales)
+
+def calls(n):
+    a = slice(0, n)
+    return [lambda: ffn.mx4_quantize(x[a].float() if n > 1 else x[a]).codes, lambda: ffn.mx4_dequantize(q, torch.float16 if n > 1 else torch.bfloat16), lambda: ffn.mx4_from_rows(codes, rows).scales,
+            lambda: ffn.mx4_linear(x[a], q), lambda: ffn.mx4_gated(x[a], q, q, torch.float16), lambda: ffn.gated_forward(x[a], w, w),
+            lambda: torch.cat([v.flatten() for v in ffn.gated_backward(dh[a], x[a], w, w, g[a], u[a])])]
+
+torch.cat([v.flatten() for v in (x[:1].float().half(), w)])       # torch's own kernels
+if not first:
+    for call in calls(1):
+        call()
+torch.cuda.synchronize()
+for i, call in enumerate(calls(tokens)):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = got.clone()
+    assert torch.equal(got, call()), i
+assert ffn.status() == 0
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("before", ["first", "another size"])
+@pytest.mark.parametrize("tokens", [1, 50, 300])
+def test_captures_of_kernels_that_have_not_run(before, tokens):
+    """Processes whose first call of every entry point is a captured one, or that have called it with one token before (which takes other kernels)."""
+    done = subprocess.run([sys.executable, "-c", CAPTURES, before, str(tokens)], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.endswith("captured\n"), done.stderr[-2000:]

@@ -9,7 +9,7 @@ its gradient - the shared or dense form of the block whose routed form is ``zero
     dx, dgate, dup = gated_backward(dh, x, gate, up, g, u)
 
 Calls run on the tensors' device and torch's current stream of it, allocate results and scratch with torch and may be captured into a
-CUDA graph (after one call outside a capture). Nothing here has a CPU path, and autograd does not see these calls: a block or product of tensors that
+CUDA graph, the first call of a process too. Nothing here has a CPU path, and autograd does not see these calls: a block or product of tensors that
 require gradients is refused where gradients are recorded, as its result would silently have none (call it under ``torch.no_grad()``, or pass
 ``x.detach()``). Errors are those of ``zerocool_b200.moe``: ``ValueError`` for arguments, ``RuntimeError`` for the device.
 """
