@@ -5,7 +5,9 @@
  *
  * Conventions (those of zc_moe.h where not stated here)
  *  - Plain C: ZC_OK or a negative code; zc_last_error() has the text. Everything is validated on the host before a launch.
- *  - No handle and no allocation: every buffer is the caller's device memory, on the current device, 16-byte aligned. Calls are
+ *  - No handle and no allocation: every buffer is the caller's device memory, on the current device. Codes, tiled scales and the buffers of the 16-bit block
+ *    are 16-byte aligned (its rows too); the plain matrices of the microscaled calls need no more than their type's alignment, and no row stride in
+ *    particular (those whose rows are 16-byte aligned are read and written in wider pieces); row-major scales need none. Calls are
  *    stream-ordered, do not block the host and may be captured into a graph (a process's first call of an entry point too: an entry point has
  *    kernels of several sizes and types, and what a capture meets first is loaded then). Calls on different streams share nothing but the status word of the device.
  *  - Row strides count elements; that of a single row has no meaning and may be anything.
@@ -32,15 +34,12 @@
 extern "C" {
 #endif
 
-#define ZC_MX4 3   /* element type beside ZC_BF16, ZC_F32, ZC_F16: a microscaled matrix */
-
 /* Bytes of the scales of a [rows, cols] matrix: ceil(rows / 128) * ceil(cols / 128) * 512. */
 int zc_mx4_scale_bytes(uint32_t rows, uint32_t cols, uint64_t* bytes);
 
 /* x [rows, cols] (dtype; row stride ld elements) -> codes, scales. Per 32 values of a row, a = their largest magnitude:
  * scale 2^e with e = floor(log2 a) - 2 (at least -127; a = 0: -127), value -> x 2^-e rounded to the nearest e2m1 value, ties to
- * the even code, magnitudes above 6 to 6. A NaN or an infinity among the 32 makes their scale 255 and their codes 0.
- * Rows that are not 16-byte aligned (ld, x) are read value by value: only here x needs no more than its type's alignment. */
+ * the even code, magnitudes above 6 to 6. A NaN or an infinity among the 32 makes their scale 255 and their codes 0. */
 int zc_mx4_quantize(const void* x, int dtype, uint32_t rows, uint32_t cols, uint64_t ld, void* codes, void* scales, void* stream);
 
 /* The values of a microscaled matrix in dtype, out row stride ld elements. BF16 and F32 hold every one below 2^128 exactly (those

@@ -220,6 +220,39 @@ def test_a_single_row_of_any_stride(ffn, ld):
     assert torch.equal(dx, want[0]) and torch.equal(dgate, want[1]) and torch.equal(got, want[2])
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 32), (3, 96), (37, 288), (130, 1056)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_plain_matrices_of_any_alignment(ffn, rows, cols, dtype):
+    """Every call that takes or gives a plain matrix of the microscaled forms, at an element's alignment: dequantisation into it, products from and into it."""
+    q, w = ffn.mx4_quantize(randn((rows, cols), 1)), ffn.mx4_quantize(randn((72, cols), 2, 0.1))
+    for left, right in ((1, 0), (3, 2), (0, 1), (8, 8), (5, 3)):
+        big = torch.full((rows + 2, cols + left + right), 7.0, dtype=dtype, device="cuda")
+        out = big[1:rows + 1, left:left + cols]
+        assert ffn.mx4_dequantize(q, out=out) is out
+        assert torch.equal(out.double(), ref.of(q).to(dtype).double())
+        product, gated = ffn.mx4_linear(out.contiguous(), w, dtype), ffn.mx4_gated(out.contiguous(), w, w, dtype)
+        into = torch.empty(rows * 72 + 3, dtype=dtype, device="cuda")[left % 4:][:rows * 72].view(rows, 72)
+        assert torch.equal(ffn.mx4_linear(out, w, out=into), product) and torch.equal(ffn.mx4_gated(out, w, w, out=into), gated)
+        out.fill_(7.0)
+        assert bool((big == 7.0).all())
+    scales = torch.empty(rows * (cols // 32) + 3, dtype=torch.uint8, device="cuda")[3:].view(rows, cols // 32)
+    scales.copy_(ref.row_scales(q))
+    assert torch.equal(ffn.mx4_from_rows(q.codes, scales).scales, q.scales)
+
+
+def test_the_gated_block_writes_where_it_is_told(ffn):
+    x, gate, up = (randn((r, 64), s, dtype=torch.float16) for s, r in ((1, 70), (2, 48), (3, 48)))
+    for tokens in (1, 40, 70):
+        big = torch.full((tokens + 2, 48), 7.0, dtype=torch.float16, device="cuda")
+        out = big[1:-1]
+        h, g, u = ffn.gated_forward(x[:tokens], gate, up, save=True, out=out)
+        assert h is out and torch.equal(h, ffn.gated_forward(x[:tokens], gate, up))
+        assert bool((big[0] == 7.0).all()) and bool((big[-1] == 7.0).all())
+        for wrong in (big, big[:, :40], big.float()[1:-1], out.t(), 3, out.cpu()):
+            with pytest.raises(ValueError):
+                ffn.gated_forward(x[:tokens], gate, up, out=wrong)
+
+
 # -- captures ------------------------------------------------------------------------------------------------------------------
 
 CAPTURES = """
