@@ -253,6 +253,55 @@ def test_the_gated_block_writes_where_it_is_told(ffn):
                 ffn.gated_forward(x[:tokens], gate, up, out=wrong)
 
 
+# -- plans that the sizes of test_ffn_gpu.py do not reach ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,rows,cols", [(19, 14300, 2080), (40, 18900, 4128), (3, 19100, 2080), (17, 14210, 8224), (32, 15000, 288), (48, 19000, 800)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_few_tokens_over_many_rows(ffn, tokens, rows, cols, dtype):
+    """As many tiles of rows as SMs: no cluster, the whole of K in one CTA, more of its blocks than the ring has stages."""
+    x, gate, up = randn((tokens, cols), 1, dtype=dtype), *(ffn.mx4_quantize(randn((rows, cols), s, 0.05)) for s in (2, 3))
+    q = ffn.mx4_quantize(x)
+    xd, gd, ud = ref.of(q), ref.of(gate), ref.of(up)
+    g, u, gs, us = xd @ gd.T, xd @ ud.T, sums(xd, gd, 64), sums(xd, ud, 64)
+    h, slack = ref.silu(g) * u, 1.1 * gs * u.abs() + ref.silu(g).abs() * us + 1.1 * gs * us + 2.0 ** -20 * (ref.silu(g) * u).abs()
+    for a in (x, q):
+        close(ffn.mx4_linear(a, gate, dtype), g, gs)
+        close(ffn.mx4_gated(a, gate, up, dtype), h, slack)
+
+
+@pytest.mark.parametrize("tokens,hidden,width", [(33, 2056, 16392), (5, 1032, 20008), (64, 4104, 14216), (48, 520, 19000)])
+def test_few_tokens_over_many_rows_in_16_bits(ffn, tokens, hidden, width):
+    for dtype in (torch.bfloat16, torch.float16):
+        x, gate, up = randn((tokens, hidden), 1, dtype=dtype), randn((width, hidden), 2, 0.1, dtype), randn((width, hidden), 3, 0.1, dtype)
+        h, g, u = ffn.gated_forward(x, gate, up, save=True)
+        xd, gd, ud = x.double(), gate.double(), up.double()
+        gw, uw, gs, us = xd @ gd.T, xd @ ud.T, sums(xd, gd, 16), sums(xd, ud, 16)
+        close(g, gw, gs)
+        close(u, uw, us)
+        close(h, ref.silu(gw) * uw, 1.1 * gs * uw.abs() + ref.silu(gw).abs() * us + 1.1 * gs * us + 2.0 ** -20 * (ref.silu(gw) * uw).abs())
+
+
+@pytest.mark.parametrize("tokens,hidden,width", [(60, 16392, 264), (5, 20008, 136), (40, 19000, 1032), (65, 520, 4104), (513, 320, 264), (2, 40, 20008), (64, 2056, 4104), (33, 264, 200),
+                                                 (129, 264, 72), (1500, 2056, 136), (200, 2056, 136), (900, 520, 1200), (1100, 264, 2600), (300, 16, 8), (1, 64, 128), (4100, 136, 72)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_are_the_products_of_dg_and_du(ffn, tokens, hidden, width, dtype):
+    """dg and du element by element against the formula, then dx, dgate and dup against the 64-bit products of the very dg and du that the call left: with
+    nothing but the sums and one rounding to allow for, a token, a column of K or a segment that is missing anywhere shows."""
+    x, gate, up = randn((tokens, hidden), 1, dtype=dtype), randn((width, hidden), 2, 0.2, dtype), randn((width, hidden), 3, 0.2, dtype)
+    g, u, dh = randn((tokens, width), 4, 2.0), randn((tokens, width), 5, 2.0), randn((tokens, width), 6, 0.5, dtype)
+    dg, du, dx, dgate, dup = gradient(ffn, dh, x, gate, up, g, u)
+    d = [t.double() for t in (dh, x, gate, up, g, u)]
+    for got, want, slack in zip((dg, du), ref.gated_gradient(*d)[:2], elementwise_slack(d[0], d[4], d[5])):
+        close(got, want, slack)
+    gd, ud, xd, wg, wu = dg.double(), du.double(), d[1], d[2], d[3]
+    close(dx, gd @ wg + ud @ wu, 2 * -(-width // 16) * 2.0 ** -22 * (gd.abs() @ wg.abs() + ud.abs() @ wu.abs()), "dx")
+    close(dgate, gd.T @ xd, sums(gd.T, xd.T, 16), "dgate")
+    close(dup, ud.T @ xd, sums(ud.T, xd.T, 16), "dup")
+    only_x, only_w = gradient(ffn, dh, x, gate, up, g, u, want_w=False), gradient(ffn, dh, x, gate, up, g, u, want_x=False)
+    assert torch.equal(only_x[2], dx) and torch.equal(only_w[3], dgate) and torch.equal(only_w[4], dup)
+    assert torch.equal(only_x[0], dg) and torch.equal(only_w[1], du)
+
+
 # -- captures ------------------------------------------------------------------------------------------------------------------
 
 CAPTURES = """
