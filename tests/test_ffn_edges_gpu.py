@@ -302,6 +302,32 @@ def test_gradients_are_the_products_of_dg_and_du(ffn, tokens, hidden, width, dty
     assert torch.equal(only_x[0], dg) and torch.equal(only_w[1], du)
 
 
+def test_beside_products_of_other_libraries(ffn):
+    """Kernels of few and of many tokens beside torch's own products of several sizes on another stream, which use tensor memory and clusters as well."""
+    w4, w16 = [ffn.mx4_quantize(randn((1024, 2048), 2 + i, 0.05)) for i in range(2)], [randn((1024, 2048), 4 + i, 0.05, torch.bfloat16) for i in range(2)]
+    jobs = []
+    for tokens in (1, 7, 40, 64, 300):
+        x = randn((tokens, 2048), tokens, dtype=torch.bfloat16)
+        g, u, dh = randn((tokens, 1024), 6), randn((tokens, 1024), 7), randn((tokens, 1024), 8, dtype=torch.bfloat16)
+        jobs += [lambda x=x: ffn.mx4_linear(x, w4[0]), lambda x=x: ffn.mx4_gated(x, *w4), lambda x=x: ffn.gated_forward(x, *w16),
+                 lambda x=x, g=g, u=u, dh=dh: ffn.gated_backward(dh, x, *w16, g, u, weight_grads=False)[0]]
+    others = [(randn((n, k), 9, dtype=torch.bfloat16), randn((k, m), 10, dtype=torch.bfloat16)) for n, k, m in ((64, 512, 512), (128, 4096, 256), (256, 1024, 1024), (512, 512, 2048), (2048, 2048, 2048))]
+    want, theirs = [job() for job in jobs], [a @ b for a, b in others]
+    torch.cuda.synchronize()
+    streams, got, kept = [torch.cuda.Stream() for _ in range(3)], [], []
+    for round_ in range(8):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[0]):
+                got.append((i, job()))
+            for s in streams[1:]:
+                with torch.cuda.stream(s):
+                    j = (i + round_) % len(others)
+                    kept.append((j, others[j][0] @ others[j][1]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    assert all(torch.allclose(y.float(), theirs[j].float(), rtol=2e-2, atol=1.0) for j, y in kept)
+
+
 # -- captures ------------------------------------------------------------------------------------------------------------------
 
 CAPTURES = """

@@ -229,7 +229,9 @@ template <int N> __device__ __forceinline__ void activate(float (&v)[N], const f
 //
 // A CTA that waits for tensor memory while others wait for it could close a circle over two SMs (two clusters, each with one CTA that has its
 // columns and one that has not). So no CTA here ever waits for another's columns: each takes at least the share of its SM's shared memory that it
-// takes of the tensor memory, so that those that fit an SM together find their columns free. A tile CTA takes all 512, hence all of the shared memory.
+// takes of the tensor memory, so that those that fit an SM together find their columns free. A tile CTA takes all 512, hence all of the shared memory: it
+// has its SM alone, whatever else runs. A CTA of few tokens may meet those of other libraries; it holds its columns while it waits for nothing
+// but its own copies and products.
 constexpr uint32_t SM_SMEM = 228 * 1024, CTA_RESERVED = 1024, CTA_STATIC = 256, CTA_SMEM_MAX = 227 * 1024 - CTA_STATIC;
 constexpr uint32_t smem_share(uint32_t tmem_columns) { return tmem_columns * (SM_SMEM / 512) - CTA_RESERVED - CTA_STATIC; }
 
@@ -790,10 +792,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant_
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    if (p.splits > 1) cluster_sync();
-    else __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
+    // The columns go back as soon as they are read, before the cluster is waited for: a kernel of another library that waits for them, on a CTA of whose
+    // cluster another CTA here waits, gets them. (The warps that read them only arrive; with a barrier of the whole CTA a call took 0.1 us more.)
+    if (warp == 1) {
+        if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("bar.sync 1, 160;" ::: "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_columns) : "memory");
+        if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        if (warp >= 2) asm volatile("bar.arrive 1, 160;" ::: "memory");
+        if (p.splits > 1) cluster_sync();
+    }
     if (p.splits > 1) {
         // Sums that are not stored are not loaded either: cluster_leave waits for no load, so each of them has to be used before it.
         const uint32_t row = lane * 4;               // four rows a lane, a token a warp
