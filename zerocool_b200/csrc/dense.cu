@@ -59,8 +59,8 @@ constexpr uint32_t SF_COLUMNS = 32;                        // MX4: tensor-memory
 
 struct TileMaps { CUtensorMap a[2], b[2], sfa, sfb[2], o[3]; };
 
-// Division of n < 2^31 by a divisor known on the host: (umulhi(mul, n) + n) >> shift with mul = 2^32 (2^shift - d) / d + 1, 2^shift >= d. The tile
-// of an index takes two; as divisions they stopped the copying thread for 1,000 clocks a tile.
+// Division of n < 2^31 by a divisor known on the host, by the method of Granlund and Montgomery ("Division by invariant integers using multiplication",
+// 1994): (umulhi(mul, n) + n) >> shift with mul = 2^32 (2^shift - d) / d + 1, 2^shift >= d. The tile of an index takes two; as divisions they stopped the copying thread for 1,000 clocks a tile.
 struct Divisor {
     uint32_t d, mul, shift;
     void set(uint32_t by) {
@@ -1002,8 +1002,11 @@ void plan_few(FewPlan& p, bool mx4, uint32_t mats, bool plain, uint32_t sms) {
     p.n = (p.tokens + 15) / 16 * 16;
     const uint32_t total = p.kblocks * p.segs, mtiles = (p.M + TILE_M - 1) / TILE_M;
     // Two CTAs an SM: 8192 x 4096, one token 6.4 us, with one CTA an SM 7.5. Where the tiles alone fill three quarters of the SMs, more than sixteen
-    // tokens are not split: their sums cost more than the second CTA brings (16384 x 2048, 19 / 64 tokens 9.2 / 11.2 us, split in two 9.8 / 12.2; one
-    // token 7.2 and 6.5).
+    // tokens are not split: their sums cost more than the second CTA brings. Rows x K, in two / in one, us, of MX4 product | MX4 block (tokens microscaled) |
+    // 16-bit block | dx: 14336 x 512, 17 tokens 5.1 / 3.6 | 7.2 / 5.9 | 9.3 / 8.6 | 10.3 / 9.3; 16384 x 2048, 17 tokens 6.7 / 5.7 | 10.2 / 9.3 |
+    // 26.6 / 25.6 | 27.7 / 26.7, 32 tokens 7.1 / 6.1 | 10.5 / 9.6 | 27.7 / 26.0; 16384 x 8192, 64 tokens 19.3 / 16.9 | 32.8 / 30.0 | 92.3 / 87.2; against
+    // the rule 18904 x 1024, 17 tokens 5.7 / 4.1 | 8.2 / 7.5 | 17.6 / 18.3 | 20.5 / 19.9. Up to sixteen it depends: 16384 x 2048, one token 5.8 / 5.7 |
+    // 8.3 / 8.3 | 24.9 / 25.0, 16 tokens of dx 26.8 / 26.2, but one plain token, of which every CTA would quantise twice as much, 5.7 / 6.2 | 8.3 / 10.7.
     uint32_t splits = p.tokens > 16 && mtiles >= sms * 3 / 4 ? 1 : 2 * sms / mtiles;
     splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
     if (splits > total) splits = total;
