@@ -328,6 +328,84 @@ def test_beside_products_of_other_libraries(ffn):
     assert all(torch.allclose(y.float(), theirs[j].float(), rtol=2e-2, atol=1.0) for j, y in kept)
 
 
+# -- the largest sizes, the same matrix twice, threads ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [1, 12, 70, 300])
+def test_the_longest_rows(ffn, tokens):
+    """K, then the rows of the weights, of 2^20."""
+    x, gate, up = randn((tokens, 1 << 20), 1), *(ffn.mx4_quantize(randn((72, 1 << 20), s, 0.01)) for s in (2, 3))
+    q = ffn.mx4_quantize(x)
+    xd, gd, ud = ref.of(q), ref.of(gate), ref.of(up)
+    g, u, gs, us = xd @ gd.T, xd @ ud.T, sums(xd, gd, 64), sums(xd, ud, 64)
+    slack = 1.1 * gs * u.abs() + ref.silu(g).abs() * us + 1.1 * gs * us + 2.0 ** -20 * (ref.silu(g) * u).abs()
+    for a in (x, q):
+        close(ffn.mx4_linear(a, gate, torch.float32), g, gs)
+        close(ffn.mx4_gated(a, gate, up, torch.float32), ref.silu(g) * u, slack)
+    x, gate = randn((tokens, 8), 1, dtype=torch.bfloat16), randn((1 << 20, 8), 2, dtype=torch.bfloat16)
+    h, g, u = ffn.gated_forward(x, gate, gate, save=True)
+    gw, gs = x.double() @ gate.double().T, sums(x.double(), gate.double(), 16)
+    close(g, gw, gs)
+    close(h, ref.silu(gw) * gw, 2.1 * gs * gw.abs() + 1.1 * gs * gs + 2.0 ** -20 * (ref.silu(gw) * gw).abs())
+    dg, du, dx, dgate, dup = gradient(ffn, h, x, gate, gate, g, u)
+    gd, ud, xd, wd = dg.double(), du.double(), x.double(), gate.double()
+    close(dx, gd @ wd + ud @ wd, 2 * (1 << 16) * 2.0 ** -22 * (gd.abs() + ud.abs()) @ wd.abs(), "dx")
+    close(dgate, gd.T @ xd, sums(gd.T, xd.T, 16), "dgate")
+    close(dup, ud.T @ xd, sums(ud.T, xd.T, 16), "dup")
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_a_matrix_with_itself(ffn, rows):
+    """x, gate and up may be one and the same."""
+    q = ffn.mx4_quantize(randn((rows, 544), 1, 0.3))
+    v = ref.of(q)
+    g, s = v @ v.T, sums(v, v, 64)
+    close(ffn.mx4_linear(q, q, torch.float32), g, s)
+    close(ffn.mx4_gated(q, q, q, torch.float32), ref.silu(g) * g, 2.1 * s * g.abs() + 1.1 * s * s + 2.0 ** -20 * (ref.silu(g) * g).abs())
+
+
+THREADS = """
+import threading, torch
+from zerocool_b200 import ffn
+torch.manual_seed(0)
+w, v = torch.randn(304, 512, device="cuda").bfloat16(), torch.randn(304, 512, device="cuda").bfloat16()
+scales = torch.randint(100, 130, (3 * 4 * 512,), device="cuda").to(torch.uint8)
+q = ffn.Mx4(torch.randint(0, 256, (304, 256), device="cuda").to(torch.uint8), scales)
+xs = [torch.randn(n, 512, device="cuda").bfloat16() for n in (1, 40, 300, 700)]
+torch.cuda.synchronize()
+start, results = threading.Barrier(len(xs)), {}
+
+def work(i, x):
+    out = []
+    start.wait()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):
+            h, g, u = ffn.gated_forward(x, w, v, save=True)
+            out.append([ffn.mx4_linear(x, q), ffn.mx4_gated(x, q, q), ffn.mx4_quantize(x).codes, h, *ffn.gated_backward(h, x, w, v, g, u)])
+            try:
+                ffn.mx4_linear(x[:, :32 + 32 * i], q)
+            except ValueError as e:
+                assert f"{32 + 32 * i} columns" in str(e)
+        torch.cuda.current_stream().synchronize()
+    results[i] = out
+
+threads = [threading.Thread(target=work, args=a) for a in enumerate(xs)]
+[t.start() for t in threads], [t.join() for t in threads]
+for i, x in enumerate(xs):
+    h, g, u = ffn.gated_forward(x, w, v, save=True)
+    want = [ffn.mx4_linear(x, q), ffn.mx4_gated(x, q, q), ffn.mx4_quantize(x).codes, h, *ffn.gated_backward(h, x, w, v, g, u)]
+    for got in results[i]:
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+assert ffn.status() == 0
+print("done")
+"""
+
+
+def test_threads_that_call_first_at_the_same_time(ffn):
+    """Four threads of a fresh process, each on a stream of its own: their first calls of every kernel meet."""
+    done = subprocess.run([sys.executable, "-c", THREADS], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.endswith("done\n"), done.stderr[-2000:]
+
+
 # -- captures ------------------------------------------------------------------------------------------------------------------
 
 CAPTURES = """
