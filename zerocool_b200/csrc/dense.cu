@@ -503,23 +503,25 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 // of it would arrive too.
 // What bounds it: one token, MX4 8192 x 4096, replayed back to back 6.1 us a call for 17.8 MB (2.7 us of HBM): 1.7 us until the first stage is there
 // (all CTAs ask for all weights at once: 10 TB/s out of L2), 1.3 for the products, 0.7 for the sums, 0.6 to leave the cluster, 1.5 until the next
-// kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 0.2 us more.
+// kernel is let go. Sums written to the ranks that add them, one cluster barrier the less, came to 0.2 us more. (With all ends of copies and products
+// waited for, 6.2.)
 constexpr uint32_t FEW_THREADS = 192;
 // Which calls: up to 64 tokens, unless K is short, where the tokens' sums over the cluster cost more than the weights. Rows x K, here / in tiles of pairs, us,
-// of MX4 product | MX4 block | 16-bit block. 2048 x 512: 25 tokens 4.1 / 4.1 | 7.5 / 7.6 | 7.2 / 7.2, 32 tokens 4.6 / 4.1 | 7.6 / 7.6 | 7.5 / 7.2, 33 tokens
-// 4.9 / 4.1 | 8.2 / 8.2 | 8.2 / 7.2, 64 tokens 6.2 / 4.4 | 10.4 / 8.2 | 9.3 / 7.2. 1024 x 1024: 48 tokens 4.6 / 4.6 | 8.2 / 8.9 | 8.3 / 8.2, 64 tokens
-// 5.3 / 4.6 | 8.9 / 8.3 | 8.3 / 8.2. 2048 x 2048: 33 tokens 5.7 / 5.4 | 8.9 / 9.6 | 9.7 / 10.3, 64 tokens 6.7 / 5.7 | 10.5 / 9.7 | 12.2 / 10.6. 1024 x 4096,
-// 64 tokens: 5.7 / 6.7 | 9.6 / 12.3 | 11.3 / 12.4. 8192 x 8192, 64 tokens: 12.5 / 14.1 | 21.9 / 22.4 | 49 / 55. What the rule gives away: few rows of K = 2048
-// (512 x 2048, 49 tokens 4.6 / 5.2 | 8.2 / 9.6 | 8.3 / 9.3; 64 tokens 5.2 / 5.2 | 8.9 / 9.6 | 9.3 / 9.3). 128 tokens of 8192 x 4096: MX4 18 / 15, 16-bit
-// block 57 / 42. dx, whose K is two segments, stays here up to 64 tokens (hidden x ffn, 2048 x 1024 8.8 / 10.3, 4096 x 4096 19 / 24, 2048 x 512 8.2 / 8.2).
+// of MX4 product | MX4 block (tokens microscaled) | 16-bit block. 2048 x 512: 25 tokens 4.1 / 3.7 | 5.7 / 6.2 | 7.2 / 7.2, 32 tokens 4.1 / 3.9 | 6.2 / 6.2 |
+// 7.3 / 7.2, 33 tokens 4.6 / 3.9 | 6.7 / 6.2 | 8.2 / 7.3, 64 tokens 5.9 / 4.1 | 8.7 / 6.2 | 9.4 / 7.2. 1024 x 1024: 48 tokens 4.4 / 4.4 | 6.5 / 6.9 | 7.3 / 8.3,
+// 64 tokens 5.1 / 4.4 | 7.2 / 6.7 | 8.2 / 8.2. 2048 x 2048: 33 tokens 5.2 / 4.9 | 7.7 / 8.2 | 9.9 / 10.3, 64 tokens 6.2 / 5.4 | 9.2 / 8.2 | 12.2 / 11.3.
+// 1024 x 4096, 64 tokens: 5.4 / 6.7 | 7.7 / 8.7 | 11.3 / 12.3. 8192 x 8192, 64 tokens: 11.8 / 13.8 | 19.5 / 19.9 | 50 / 55. One rule for forms that cross over
+// at different places; what it gives away: the MX4 product above (2048 x 2048, 33 tokens), few rows of K = 2048 (512 x 2048, 49 tokens 4.6 / 4.9 | 6.7 / 8.0 |
+// 8.3 / 8.2; 64 tokens 4.9 / 5.1 | 7.2 / 8.2 | 9.3 / 8.2). dx, whose K is two segments, stays here up to 64 tokens (hidden x ffn, 2048 x 1024 9.3 / 11.3,
+// 4096 x 4096 20 / 26, 2048 x 512 8.3 / 9.3).
 constexpr uint32_t FEW_TOKENS = 64;
 bool takes_few(uint32_t tokens, uint32_t k) { return tokens <= 32 || (tokens <= 48 && k > 512) || (tokens <= FEW_TOKENS && k > 2048); }
 // What a ring may take where SMs have two CTAs, and its stages at most. A CTA that has its SM alone takes what there is (16-bit block of 16384 x 4096,
 // 64 tokens: two stages 65 us, five 52), unless it is one of a cluster: sixteen clusters of eight such do not all fit (2048 x 2048: 9.9 us, 6.5).
 constexpr uint32_t FEW_SMEM = 110 * 1024, FEW_STAGES = 6;
 // x is quantised inside where a CTA has at most so many rows of 256 of its columns (tokens x blocks; the four warps share them): MX4 2048 x 512, one block a
-// CTA, 1 / 4 / 8 / 12 / 16 tokens 3.4 / 3.6 / 4.3 / 4.8 / 5.3 us, by a launch of its own 4.6 / 4.8 / 4.8 / 5.0 / 5.2; 8192 x 4096, four blocks, 2 / 3 / 4
-// tokens 7.2 / 7.7 / 8.5 and 8.2 / 8.5 / 8.6.
+// CTA, 1 / 4 / 8 / 12 / 16 tokens 3.1 / 3.2 / 4.0 / 4.7 / 5.2 us, by a launch of its own 4.1 / 4.1 / 4.2 / 4.7 / 4.9; 8192 x 4096, four blocks, 2 / 3 / 4
+// tokens 7.0 / 7.6 / 8.2 and 8.2 / 8.4 / 8.4.
 constexpr uint32_t FEW_PLAIN_ROWS = 12;
 constexpr uint64_t FEW_AHEAD = 32ull << 20;                               // bytes of weights requested into L2 before the kernel before has ended
 
@@ -975,9 +977,9 @@ template <bool MX4, bool A_MN, bool B_MN, bool GATED, int N> int launch_tiles(Ti
     p.polls = wait_polls.load(std::memory_order_relaxed);
     const uint32_t pairs = d.sms / 2, total = p.segs * p.kblocks;
     // K is shared by four or two pairs where all of the tiles still run at once and it is long enough to pay for the sums: narrow tiles, four pairs
-    // from 12 stages on (16-bit 256 x 2048 x 512 8.9 us, shared by none 9.9; of 8 stages 8.3 by two and 7.6), two from 18 (512 x 3000 x 1000 15.1 and
-    // 19.1; of 12 stages 10.3 and 9.4); wide ones, whose sums are twice as many, 16 (MX4 gated 300 x 4000 x 600 11.9 and 12.8) and 32
-    // (of 16 stages 13.0 and 11.1).
+    // from 12 stages on (16-bit 256 x 2048 x 512, 16 stages 8.6 us, shared by none 9.8; of 12 stages 8.3 and 8.7; of 8 stages 7.8 and 7.2), two from 18
+    // (512 x 3000 x 1000, 24 stages 14.5 and 18.6; of 20 stages 11.3 and 12.3; of 12 stages 9.8 and 9.2); wide ones, whose sums are twice as many, 16 (MX4
+    // gated 300 x 4000 x 600 11.3 and 12.8; of 8 stages 10.1 and 8.7) and 32 (512 x 8192 x 1536 15.0 and 16.4; of 16 stages 12.3 and 10.9).
     typedef TileSmem<MX4, GATED, N> Smem;
     p.splits = 1;
     if (Smem::shared && p.tiles <= configured.clusters[d.index][1] && total >= (Smem::depth == 2 ? 12 : 16)) p.splits = 4;
