@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from tests import mx4_reference as ref
-from tests.test_ffn_gpu import HALF, TINY, close, ffn, gen, randn, sums, view_of  # noqa: F401
+from tests.test_ffn_gpu import close, ffn, randn, sums, view_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))

@@ -1217,7 +1217,7 @@ int zc_gated_backward(const void* dh, uint64_t dh_ld, const void* x, uint64_t x_
     if (!tokens) {
         for (void* v : {dgate, dup}) {
             const cudaError_t e = v ? cudaMemsetAsync(v, 0, fh, s) : cudaSuccess;
-            if (e != cudaSuccess) return fail(nullptr, ZC_EEXEC, std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+            if (e != cudaSuccess) { cudaGetLastError(); return fail(nullptr, ZC_EEXEC, std::string("cudaMemsetAsync: ") + cudaGetErrorString(e)); }
         }
         return ZC_OK;
     }
